@@ -185,9 +185,10 @@ def _prepare_own(c, seed):
         k, v = _kv(c, seed, b, T)
         # what the sequence holds before the call: all but a step's or a write's new rows
         held = T - (c["new"] if write or step else 0)
-        hop = 512 if c["window"] else max(held, 1)
-        for t in range(0, held, hop):
-            n = min(hop, held - t)
+        # (a windowed pool drops what the rows appended next do not see: the chunk comes in one append)
+        chunk = held - c["new"] if c["window"] else 0
+        at = [*range(0, chunk, 512), *([chunk] if held else []), held]
+        for t, n in zip(at, np.diff(at).tolist()):
             sl = _i32(pool.reserve_append(s, n).reshape(1, n))
             pool.quantize_append(0, k[None, :, t:t + n].contiguous(), v[None, :, t:t + n].contiguous(), sl)
         if write or step:
