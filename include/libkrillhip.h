@@ -1,5 +1,5 @@
 /*
- * libkrillhip.h -- C ABI of the MI355X (gfx950) int8 paged KV-cache library.
+ * libkrillhip.h -- C ABI of the MI355X (gfx950) int8 and 4-bit paged KV-cache library.
  *
  * Drop-in for Krill's int8 KV hot path.  Each entry point names the reference
  * interface it replaces (paths relative to the srvsngh99/Krill source tree):
@@ -54,6 +54,13 @@ extern "C" {
                                  fp16 scale + fp16 zero (QuantizedKVCache.swift:181-197) */
 #define KRILL_QUANT_AFFINE_G64 1 /* affine 8-bit in groups of 64, fp16 scale + fp16 bias
                                     (MLX affine quantize semantics, CheckpointQuantizer.swift:255-260) */
+#define KRILL_QUANT_AFFINE4_G64 2 /* affine 4-bit in groups of 64, fp16 scale s and bias b: with w the group's
+                                     elements limited to +-65504, b = f16(min w), s = f16(max(0, (max w - b) / 15)),
+                                     code = min(15, max(0, rint((w - b) / s))), 0 where s = 0; a code stands for
+                                     s * code + b.  A NaN makes its group NaN.  head_dim + head_dim / 8 bytes per
+                                     token and KV head.  Every call below takes such a pool but krill_gather and
+                                     krill_scatter (KRILL_E_UNSUPPORTED: snapshots hold bytes); the limits given
+                                     for the int8 decode kernel's rows and windows do not hold for it */
 
 /* element types */
 #define KRILL_DTYPE_F16 0
@@ -71,7 +78,9 @@ extern "C" {
                                     "VALU" names the decode kernel (one token per lane for the softmax; its
                                     scores and P.V use the matrix cores at head_dim 128 with 3-8 rows and at
                                     head_dim 512), "MFMA" the row-tiled kernels of verify (9-64 rows) and of
-                                    longer query windows, which head_dim 512 takes under 0 only */
+                                    longer query windows, which head_dim 512 takes under 0 only.  4-bit pools
+                                    have two kernels: 1 keeps query windows off the one for long windows, 2 runs
+                                    every call of more than one new row on it */
 #define KRILL_OPT_WINDOW 3       /* sliding window in tokens (0 none, else >= 2): before each append a
                                     sequence keeps its last window - 1 tokens and its blocks that hold none
                                     of them go back to the pool (RotatingKVCache.trimForAppend,
@@ -263,6 +272,12 @@ int32_t krill_gather(krill_pool_t pool, int32_t layer, const int32_t *dev_block_
 int32_t krill_gather_dequant(krill_pool_t pool, int32_t layer, const int32_t *dev_block_tables,
                              const int32_t *dev_seq_lens, int32_t B, int32_t max_blocks, int32_t S_out,
                              int32_t left_pad, void *dev_k_out, void *dev_v_out, krill_stream_t stream);
+/* Read-back by slots, the inverse of krill_quantize_append: fp16 K/V
+ * [B][Hkv][L][D], row (b, l) what the cache holds at dev_slot_mapping[b][l]
+ * (values as krill_gather_dequant returns them; zeros for a slot < 0 or past
+ * the pool).  No counterpart in the reference, whose caches are read whole. */
+int32_t krill_read_slots(krill_pool_t pool, int32_t layer, const int32_t *dev_slot_mapping, int32_t B, int32_t L,
+                         void *dev_k_out, void *dev_v_out, krill_stream_t stream);
 /* Contiguous snapshot -> paged: restoreQuantized(_:) (QuantizedKVCache.swift
  * :122-129) and the int8 scatterBack slice (ContinuousBatcher.swift:743-801).
  * Row b copies snapshot tokens [dev_src_start[b], +L) to dev_slot_mapping[b][0..L). */

@@ -28,6 +28,7 @@ KRILL_E_UNSUPPORTED = -6
 
 QUANT_REF_ROW = 0
 QUANT_AFFINE_G64 = 1
+QUANT_AFFINE4_G64 = 2
 
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
@@ -156,6 +157,7 @@ SIGNATURES = {
     "krill_quantize_append_rope": [P, I32, P, P, I64, I64, I64, P, P, P, I32, I32, I32, P],
     "krill_gather": [P, I32, P, P, I32, I32, I32, I32, ctypes.POINTER(Snapshot), P],
     "krill_gather_dequant": [P, I32, P, P, I32, I32, I32, I32, P, P, P],
+    "krill_read_slots": [P, I32, P, I32, I32, P, P, P],
     "krill_scatter": [P, I32, ctypes.POINTER(Snapshot), I32, I32, P, P, I32, P],
     "krill_copy_blocks": [P, P, I32, P],
     "krill_attention_workspace_size": [P, I32, I32, I32, I32, ctypes.POINTER(ctypes.c_size_t)],

@@ -130,7 +130,7 @@ class PagedQuantizedKVCache:
         """memorySizeBytes (QuantizedKVCache.swift:33-42) for this layer."""
         n = self.sequence_length
         p = self.s.pool
-        return 2 * n * p.num_kv_heads * p.head_dim + 4 * n * p.num_kv_heads * p.groups * 2
+        return 2 * n * p.num_kv_heads * p.head_dim * p.code_bits // 8 + 4 * n * p.num_kv_heads * p.groups * 2
 
     def append(self, keys, values):
         """Quantize + append [1, Hkv, L, D] without dequantizing the cache."""
@@ -232,6 +232,8 @@ class PrefixCache:
         self.pool = pool
         self.model_id = model_id
         self.min_prefix_len = min_prefix_len  # the pool's min_prefix_len (PrefixCache minPrefixLength)
+        if cache_dir is not None and pool.code_bits != 8:
+            raise ValueError("the disk tier's files hold bytes: no cache_dir for a 4-bit pool")
         self.disk = DiskTier(cache_dir, disk_budget_gb) if cache_dir is not None else None
         gb = max_entry_gb if max_entry_gb is not None else _env_gb("KRILL_PREFIX_CACHE_MAX_ENTRY_GB")
         gb = 4.0 if gb is None else gb
@@ -254,7 +256,7 @@ class PrefixCache:
 
     def _entry_bytes(self, n: int) -> int:
         p = self.pool
-        return p.num_layers * p.num_kv_heads * n * (2 * p.head_dim + 8 * p.groups)
+        return p.num_layers * p.num_kv_heads * n * (2 * p.head_dim * p.code_bits // 8 + 8 * p.groups)
 
     def store_quantized(self, tokens, seq: int, media_hash=None) -> bool:
         """storeQuantized (PrefixCache.swift:369-400): memory entry, then the file."""

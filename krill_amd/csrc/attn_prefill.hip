@@ -34,6 +34,7 @@
 #include <type_traits>
 
 #include "attn_common.hpp"
+#include "kdev4.hpp"
 
 namespace krill {
 
@@ -42,10 +43,10 @@ namespace krill {
 // different banks), and the blocks' scales.
 template <int D, int MODE>
 struct PrefillLds {
-  static constexpr int G = MODE == MODE_AFFINE ? D / 64 : 1;
+  static constexpr int G = MODE != MODE_REF ? D / 64 : 1;
   static constexpr int KTS = D * 2 + 16, VTS = 64 * 2 + 16;
   static constexpr int GZ = (G + 3) / 4 * 4;  // groups of the zero-point contraction
-  static constexpr bool AFF = MODE == MODE_AFFINE;
+  static constexpr bool AFF = MODE != MODE_REF;
   __attribute__((aligned(16))) uint8_t k[64 * KTS];
   __attribute__((aligned(16))) uint8_t v[D * VTS];
   __attribute__((aligned(16))) float ks[AFF ? G * 64 : 4];      // [g][token]: s times the softmax scale
@@ -137,18 +138,20 @@ constexpr int prefill_min_waves() { return NRT * D >= 512 ? 1 : 2; }
 // VAR: 0 plain; 1 RoPE of the queries; 2 sliding window.
 template <int D, int MODE, int NRT, int VAR>
 __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_prefill(AttnArgs a) {
-  constexpr bool ROPE = VAR == 1, WIN = VAR == 2, AFF = MODE == MODE_AFFINE;
+  constexpr bool ROPE = VAR == 1, WIN = VAR == 2, AFF = MODE != MODE_REF, Q4 = MODE == MODE_AFFINE4;
   constexpr int G = AFF ? D / 64 : 1;
   constexpr int GZ4 = (G + 3) / 4;
   constexpr int KS = D / 32;      // 32-d steps of Q.K^T
   constexpr int NDT = D / 16;     // 16-d tiles of P.V
   constexpr int W = kPrefillWaves;
   constexpr int RR = 16 * NRT;    // query rows per wave
-  constexpr int KP = D / 16 / W;  // 16-byte K pieces per thread
-  constexpr int VP = D / 16 / W;  // 16-byte V pieces per thread
+  // 16-byte pieces per thread of K and of V (4 bits: of both, wave wid the pieces
+  // wid + W k of the region's D / 16, K's before V's)
+  constexpr int KP = D / 16 / W;
+  constexpr int VP = Q4 ? 0 : D / 16 / W;
   constexpr int MW = AFF ? (128 * G + 64 * W - 1) / (64 * W) : 0;  // metadata words per thread
   static_assert(W == 4 && D % 64 == 0, "a wave per (token group, half) of V");
-  static_assert(prefill_loads_inside<D, G>(KP, VP, MW), "a block's loads stay in its head region");
+  static_assert(Q4 || prefill_loads_inside<D, G>(KP, VP, MW), "a block's loads stay in its head region");
   using Lds = PrefillLds<D, MODE>;
   constexpr int KTS = Lds::KTS, VTS = Lds::VTS;
   __shared__ Lds lds;
@@ -226,7 +229,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
   // `lane`; V piece k holds positions 16 h .. +15 of token group tg, row d =
   // 64 k + lane, the same (tg, h) for all pieces of a wave
   const int vtg = (wid >> 1) & 1, vh = wid & 1;
-  uint4 kraw[KP], vraw[VP];
+  uint4 kraw[KP], vraw[VP > 0 ? VP : 1];
   uint32_t mraw[AFF ? MW : 1];  // affine: words tid + 64 W k of the block's metadata; row mode: K word of token `lane`
   uint32_t vmeta = 0u;          // row mode: V word of token `lane`
   const int vlane = prefill_v_lane<D>(lane);
@@ -242,13 +245,14 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
       return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, soff, 0));
     };
 #pragma unroll
-    for (int k = 0; k < KP; ++k) kraw[k] = ld16(lane * 16, prefill_k_piece(wid, k));
+    for (int k = 0; k < KP; ++k) kraw[k] = ld16(lane * 16, prefill_k_piece(wid, k));  // (4 bits: K's and V's)
 #pragma unroll
     for (int k = 0; k < VP; ++k) vraw[k] = ld16(vlane, prefill_v_piece<D>(wid, k));
     if constexpr (AFF) {
 #pragma unroll
       for (int k = 0; k < MW; ++k)
-        mraw[k] = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, prefill_meta_piece<D, G>(wid, k), 0);
+        mraw[k] = __builtin_amdgcn_raw_buffer_load_b32(
+            r, lane * 4, prefill_meta_piece<D, G>(wid, k) - (Q4 ? km_offset(D) - q4_km_offset(D) : 0), 0);
     } else {
       mraw[0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, km_offset(D), 0);
       vmeta = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, vm_offset(D, G), 0);
@@ -263,6 +267,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
   float q_up[AFF ? 1 : NRT];
   float q_dn[AFF ? NRT : 1];  // affine: 2^-k alone
   bool any_up = false;        // affine: some row of the wave has a 2^k other than 1
+  float q_bad[AFF ? NRT : 1]; // affine: NaN where the row holds an infinity or NaN, else 0
   bool rvalid[NRT];
 #pragma unroll
   for (int rt = 0; rt < NRT; ++rt) rvalid[rt] = rbase + 16 * rt + n < a.NR;
@@ -320,7 +325,10 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
         down = q_range_scale(mx, up);
       }
       q_up[rt] = qscale * up;
-      if constexpr (AFF) q_dn[rt] = down;
+      // (4 bits: rows past about 2^95 take their scores some powers of two too small,
+      // so that nothing overflows; scores that differ do so by far more than the
+      // softmax resolves either way)
+      if constexpr (AFF) q_dn[rt] = Q4 ? fmaxf(down, 0x1p-80f) : down;
       ups |= up != 1.0f;
       float qsum[G];
 #pragma unroll
@@ -354,6 +362,10 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
           qsum[g] += shfl_xor(qsum[g], 16);
           qsum[g] += shfl_xor(qsum[g], 32);
         }
+        float bad = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) bad += qsum[g] * 0.0f;
+        q_bad[rt] = bad;
 #pragma unroll
         for (int j4 = 0; j4 < GZ4; ++j4) {
           float v = 0.0f;
@@ -448,7 +460,34 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
       // here instead of held in registers through the products)
       int ln = lane;
       asm volatile("" : "+v"(ln));
-      if constexpr (AFF) {
+      if constexpr (Q4) {
+        // the layout's words are operands: eight dims of a token (K), eight tokens
+        // of two dims (V)
+        const int nn = ln & 15, qq = ln >> 4;
+#pragma unroll
+        for (int k = 0; k < KP; ++k) {
+          const int piece = wid + W * k;
+          const uint32_t w4[4] = {kraw[k].x, kraw[k].y, kraw[k].z, kraw[k].w};
+          if (piece < D / 32) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int tg = D == 64 ? 2 * piece + (w >> 1) : piece / (D / 128);
+              const int g = D == 64 ? 0 : 2 * (piece % (D / 128)) + (w >> 1);
+              *reinterpret_cast<half8_t *>(lds.k + (16 * tg + nn) * KTS + (64 * g + 16 * qq + 8 * (w & 1)) * 2) =
+                  q4_k_operand(w4[w]);
+            }
+          } else {
+            uint8_t *o = lds.v + (32 * (piece - D / 32) + nn) * VTS + 16 * qq;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+              half8_t lo, hi;
+              q4_v_operands(w4[2 * ks], w4[2 * ks + 1], lo, hi);
+              *reinterpret_cast<half8_t *>(o + 64 * ks) = lo;
+              *reinterpret_cast<half8_t *>(o + 16 * VTS + 64 * ks) = hi;
+            }
+          }
+        }
+      } else if constexpr (AFF) {
 #pragma unroll
         for (int k = 0; k < KP; ++k) {
           uint8_t *o = lds.k + ln * KTS + (wid + W * k) * 32;
@@ -461,12 +500,16 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
           *reinterpret_cast<half8_t *>(o) = bytes8_centred(uint2{vraw[k].x, vraw[k].y});
           *reinterpret_cast<half8_t *>(o + 16) = bytes8_centred(uint2{vraw[k].z, vraw[k].w});
         }
+      }
+      if constexpr (AFF) {
 #pragma unroll
         for (int k = 0; k < MW; ++k) {
           const int m = 64 * wid + ln + 64 * W * k;
           const int mm = m & (64 * G - 1), t = mm / G, g = mm % G;
           const _Float16 sh = __builtin_bit_cast(_Float16, (uint16_t)(mraw[k] & 0xffffu));
-          const float sf = (float)sh, zf = fmaf(128.0f, sf, f16_bits_to_f32((uint16_t)(mraw[k] >> 16)));
+          const float sf = (float)sh, zr = f16_bits_to_f32((uint16_t)(mraw[k] >> 16));
+          // (4 bits: K's operands are 16 + c, V's c - 8)
+          const float zf = fmaf(!Q4 ? 128.0f : m < 64 * G ? -16.0f : 8.0f, sf, zr);
           if (m < 64 * G) {
             lds.ks[g * 64 + t] = sf * a.scale_log2;
             lds.kz[g * 64 + t] = zf * a.scale_log2;
@@ -769,7 +812,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
         float c = c_part[rt][g];
         c += shfl_xor(c, 16);
         c += shfl_xor(c, 32);
-        cg[g] = c;
+        cg[g] = AFF ? c + q_bad[AFF ? rt : 0] : c;  // (a NaN score would be lost in the running reference)
       }
       if (!rvalid[rt]) continue;
       const float mul = !whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
@@ -780,7 +823,11 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
         for (int dt = 0; dt < NDT; ++dt) {
           float run[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) run[x] = (oacc[rt][dt][x] + cg[AFF ? dt / 4 : 0]) * mul;
+          for (int x = 0; x < 4; ++x) {
+            // (4 bits: odd tiles' codes came times 16)
+            const float o = Q4 && (dt & 1) ? oacc[rt][dt][x] * 0.0625f : oacc[rt][dt][x];
+            run[x] = (o + cg[AFF ? dt / 4 : 0]) * mul;
+          }
           store_run<4>(out, ob + 16 * dt, run, decltype(dtype)::value);
         }
       };
@@ -843,6 +890,15 @@ hipError_t launch_attn_prefill(const PoolGeometry &g, int32_t layer, const AttnL
   const int64_t groups = (p.row_groups + p.group_waves - 1) / p.group_waves;
   if ((int64_t)p.waves * g.Hkv * groups > INT32_MAX) return hipErrorInvalidValue;
   const AttnArgs args = make_attn_args(g, layer, a, p);
+  if (g.mode == MODE_AFFINE4) {
+    switch (g.D) {
+      case 64: return launch_prefill_dm<64, MODE_AFFINE4>(args, p, st);
+      case 128: return launch_prefill_dm<128, MODE_AFFINE4>(args, p, st);
+      case 256: return launch_prefill_dm<256, MODE_AFFINE4>(args, p, st);
+      case 512: return launch_prefill_dm<512, MODE_AFFINE4>(args, p, st);
+      default: return hipErrorInvalidValue;
+    }
+  }
   switch (g.D) {
     case 64:
       return g.mode == MODE_REF ? launch_prefill_dm<64, MODE_REF>(args, p, st)

@@ -1,0 +1,723 @@
+// Attention over the 4-bit paged KV cache for up to a few dozen query rows per
+// KV head: decode steps (with the step's append, RoPE and sliding windows) and
+// speculative verification.
+//
+//   o_j = sum_t p_jt v_t / sum_t p_jt,  p_jt = 2^(x_jt - m_j),
+//   x_jt = scale log2(e) q_j . k_t,  k_t, v_t = s c + b per group of 64 dims
+//
+// in one pass over the blocks with a running reference m, so a block's bytes go
+// from HBM to registers once and nothing is dequantized:
+//   x = f sum_g s_g (q' . (16 + c))_g + sum_g (b_g - 16 s_g) Z_g,   Z_g = scale log2(e) sum_g q
+//   o = sum_g [ sum_t (p_t s_tg) (c_t - 8) + sum_t p_t (b_tg + 8 s_tg) ]
+// Codes become matrix operands in one or two instructions per pair, from words
+// loaded in the operands' order (kdev4.hpp): one wave holds 16
+// rows (query positions x heads of the KV group) in the columns of
+// v_mfma_f32_16x16x32_f16, K tiles of 16 tokens and V tiles of 16 dims in its
+// rows; the tiles S^T = K . Q^T leave a lane four tokens of one row, which is
+// where O^T += V^T . P^T wants them, so P stays in registers.
+//
+// Numerics: queries are scaled by a power of two per row and held in fp16
+// (exact for bf16 and fp16 inputs down to 2^-25 of the row's largest), sums and
+// the softmax in fp32; a weight p s is split into an fp16 high part and the fp16
+// rounding of the rest (2^-22 of it), two products.
+//
+// Work split: the flat order of the int8 kernels -- per (KV head, row group) the
+// blocks of all sequences end to end, the same number to every wave -- and their
+// merge of partial results.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_common.hpp"
+#include "kdev4.hpp"
+
+namespace krill {
+
+namespace {
+
+// Per-wave LDS: the block's metadata words [group][token] (V: zero where the
+// token is not the sequence's), the codes and words of the step's new token.
+template <int D>
+struct Q4Lds {
+  static constexpr int G = D / 64;
+  __attribute__((aligned(16))) uint32_t km[64 * G];
+  __attribute__((aligned(16))) uint32_t vm[64 * G];
+  __attribute__((aligned(16))) uint8_t newk[D], newv[D];  // a code per byte
+  uint32_t newkm[G], newvm[G];
+};
+
+// LDS of one wave: its operations complete in order, waiting for them orders its
+// lanes' writes before other lanes' reads.
+__device__ __forceinline__ void wave_sync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t word_of(const uint4 &v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
+__device__ __forceinline__ void set_word(uint4 &v, int w, uint32_t x) {
+  (w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w) = x;
+}
+__device__ __forceinline__ float lo_f32(uint32_t w) { return f16_bits_to_f32((uint16_t)(w & 0xffffu)); }
+__device__ __forceinline__ float hi_f32(uint32_t w) { return f16_bits_to_f32((uint16_t)(w >> 16)); }
+
+// A raised reference lies kGap below the row's maximum, and is raised when a
+// score exceeds it by kOver: p < 2^8, and p s_v is finite in fp16 for |s_v| <=
+// kBig.  A block with a larger scale raises it to the maximum itself (p <= 1;
+// the quantizer's scales are below 8740).
+constexpr float kGap = 5.0f, kOver = 8.0f, kBig = 255.0f;
+
+// Waves per SIMD the registers are budgeted for.
+template <int D, int NRT>
+constexpr int q4_waves() { return D * NRT >= 512 ? 1 : 2; }
+
+// One row of K or V (lane: E = D/64 consecutive dims, fp32) as codes: the wave's
+// form of the append kernel's quantizer.
+template <int D, int DT>
+__device__ __forceinline__ uint32_t q4_quantize_row(const float (&x)[D / 64], uint32_t (&code)[D / 64]) {
+  constexpr int E = D / 64, LPG = 64 / E;
+  float w[E], lo = INFINITY, hi = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    nan |= x[e] != x[e];
+    w[e] = q4_limit<DT>(x[e]);
+    lo = fminf(lo, w[e]);
+    hi = fmaxf(hi, w[e]);
+  }
+  lo = wave_min_range<1, LPG / 2>(lo);
+  hi = wave_max_range<1, LPG / 2>(hi);
+  const uint64_t in_group = (LPG == 64 ? ~0ull : ((1ull << (LPG & 63)) - 1)) << ((threadIdx.x & 63) / LPG * LPG);
+  const bool any = (__ballot(nan) & in_group) != 0;
+  float s, b;
+  const uint32_t meta = q4_params(lo, hi, any, s, b);
+  const float r = __builtin_amdgcn_rcpf(s);
+#pragma unroll
+  for (int e = 0; e < E; ++e) code[e] = q4_code(w[e], s, b, r);
+  return meta;
+}
+
+}  // namespace
+
+// NRT: tiles of 16 query rows per wave.  WIN: sliding window.
+template <int D, int NRT, bool WIN>
+__global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a) {
+  constexpr int G = D / 64;
+  constexpr int NP = D / 32;   // 16-byte pieces per lane of K, and of V
+  constexpr int NDT = D / 16;  // 16-dim tiles of the output
+  constexpr int RR = 16 * NRT;
+  constexpr int E = D / 64;
+  __shared__ Q4Lds<D> lds;
+
+  const int lane = threadIdx.x & 63, n = lane & 15, q4 = lane >> 4;
+  const int hk = blockIdx.y, rg = blockIdx.z;
+  // (range w of the heads goes to different XCDs)
+  const int wv = (int)((blockIdx.x + (unsigned)hk) % gridDim.x);
+  const int rbase = rg * RR;
+
+  // ---- flat blocks [i0, iend) of the (head, row group) order
+  int c0 = 0, lenv = lane < a.B ? seq_len_view<WIN>(a, lane) : 0;
+  int nbv = seq_blocks_rg(a, lenv, rg);
+  int incl = wave_incl_scan(nbv);
+  int T = __builtin_amdgcn_readlane(incl, 63);
+  for (int cc = 64; cc < a.B; cc += 64) {
+    const int bb = cc + lane;
+    T += __builtin_amdgcn_readfirstlane(wave_allsum_int(bb < a.B ? seq_blocks_rg(a, seq_len_view<WIN>(a, bb), rg) : 0));
+  }
+  // (every wave that takes part holds a block: the merge relies on it)
+  const int Wt = min(a.waves, T);
+  if (wv >= Wt) return;
+  const int i0 = __builtin_amdgcn_readfirstlane((int)(((int64_t)wv * T + Wt - 1) / Wt));
+  const int iend = __builtin_amdgcn_readfirstlane((int)(((int64_t)(wv + 1) * T + Wt - 1) / Wt));
+  int b = -1, s = 0;  // the sequence of block i0, the flat index of its first block
+  {
+    int carry = 0;
+    for (c0 = 0; c0 < a.B; c0 += 64) {
+      if (c0 > 0) {
+        const int bb = c0 + lane;
+        lenv = bb < a.B ? seq_len_view<WIN>(a, bb) : 0;
+        nbv = seq_blocks_rg(a, lenv, rg);
+        incl = wave_incl_scan(nbv) + carry;
+      }
+      const unsigned long long m = __ballot(c0 + lane < a.B && incl > i0);
+      if (m) {
+        const int l = __builtin_ctzll(m);
+        b = c0 + l;
+        s = __builtin_amdgcn_readlane(incl - nbv, l);
+        break;
+      }
+      carry = __builtin_amdgcn_readlane(incl, 63);
+    }
+  }
+  if (b < 0) return;
+  auto seq_len = [&](int bs) -> int { return bs - c0 < 64 ? __builtin_amdgcn_readlane(lenv, bs - c0) : seq_len_view<WIN>(a, bs); };
+
+  // block-table entries of flat blocks tab0 .. tab0 + 63, one a lane (-1: none
+  // of the pool's); reloaded every 64 blocks, walking on from sequence b
+  int tab = -1, tab0 = i0;
+  auto load_table = [&](int from) {
+    const int f = from + lane;
+    int bs = b, ss = s;
+    tab = -1;
+    while (bs < a.B && ss < min(iend, from + 64)) {
+      const int nbs = seq_blocks_rg(a, seq_len(bs), rg);
+      if (f < iend && f >= ss && f < ss + nbs) {
+        const int phys = a.tables[(int64_t)bs * a.max_blocks + table_offset<WIN>(a, bs) + (f - ss)];
+        tab = (unsigned)phys < (unsigned)a.lv.num_blocks ? phys : -1;
+      }
+      ss += nbs;
+      ++bs;
+    }
+    tab0 = from;
+  };
+  load_table(i0);
+
+  // ---- a block in registers; blocks past the range and outside the pool read as
+  // zeros without touching memory
+  uint4 kq[NP], vq[NP];
+  uint32_t mk[G], mv[G];  // words of token `lane`
+  auto rsrc_of = [&](int i) -> __amdgpu_buffer_rsrc_t {
+    const int phys = __builtin_amdgcn_readlane(tab, __builtin_amdgcn_readfirstlane((i - tab0) & 63));
+    const bool ok = i < iend && phys >= 0;
+    return block_rsrc(head_region(a.lv, ok ? phys : 0, hk), ok ? a.lv.head_bytes : 0);
+  };
+  auto ld16 = [](__amdgpu_buffer_rsrc_t r, int off) {
+    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 2));
+  };
+  auto ld_words = [](__amdgpu_buffer_rsrc_t r, int off, uint32_t (&w)[G]) {
+    if constexpr (G == 1) {
+      w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 2);
+    } else if constexpr (G == 2) {
+      const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 2);
+      w[0] = v[0];
+      w[1] = v[1];
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; g += 4) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * g, 0, 2);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[g + k] = v[k];
+      }
+    }
+  };
+  auto load_k = [&](__amdgpu_buffer_rsrc_t r) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) kq[p] = ld16(r, p * 1024 + lane * 16);
+    ld_words(r, q4_km_offset(D) + lane * G * 4, mk);
+    ld_words(r, q4_vm_offset(D) + lane * G * 4, mv);
+  };
+  auto load_v = [&](__amdgpu_buffer_rsrc_t r) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) vq[p] = ld16(r, q4_v_offset(D) + p * 1024 + lane * 16);
+  };
+
+  // ---- queries of sequence bq: lane (n, q4) holds dims 64 g + 16 q4 + 8 h .. +7
+  // of row n in qB[..][2 g + h]
+  half8_t qB[NRT][2 * G];
+  float Z[NRT][G];  // scale log2(e) times the row's sum over group g
+  float fr[NRT];    // what a sum of products takes
+  bool rvalid[NRT];
+#pragma unroll
+  for (int rt = 0; rt < NRT; ++rt) rvalid[rt] = rbase + 16 * rt + n < a.NR;
+  auto load_q = [&](int bq) {
+#pragma unroll
+    for (int rt = 0; rt < NRT; ++rt) {
+      const int r = rvalid[rt] ? rbase + 16 * rt + n : 0;
+      const int hq = hk * a.R + r % a.R, j = r / a.R;
+      const uint16_t *qp = q_row(a, bq, hq, j) + 16 * q4;
+      uint4 raw[2 * G];
+#pragma unroll
+      for (int k = 0; k < 2 * G; ++k) raw[k] = *reinterpret_cast<const uint4 *>(qp + 64 * (k >> 1) + 8 * (k & 1));
+      if (a.rope_cs) {
+        // dim d < D/2 turns with d + D/2: the same lane's operand G later, or
+        // (head_dim 64) lane ^ 32's
+        const int len = WIN ? len_of(a, bq) : seq_len(bq);  // absolute positions
+        const float *crow = rope_row(a, len - a.Lq + j, D) + (D == 64 ? 16 * (q4 & 1) : 16 * q4);
+#pragma unroll
+        for (int k = 0; k < (D == 64 ? 2 : G); ++k) {
+          uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w}, y[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            y[w] = D == 64 ? (uint32_t)__shfl_xor((int)x[w], 32, 64) : word_of(raw[D == 64 ? 0 : k + G], w);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float *cp = crow + 64 * (k >> 1) + 8 * (k & 1) + 2 * w;
+            const float2 c2 = *reinterpret_cast<const float2 *>(cp), s2 = *reinterpret_cast<const float2 *>(cp + D / 2);
+            const bool up = D == 64 && q4 >= 2;
+            uint32_t lo = up ? y[w] : x[w], hi = up ? x[w] : y[w];
+            if (a.q_dtype == DT_BF16)
+              rope_pair_words<DT_BF16>(lo, hi, c2, s2);
+            else
+              rope_pair_words<DT_F16>(lo, hi, c2, s2);
+            x[w] = up ? hi : lo;
+            y[w] = up ? lo : hi;
+          }
+          raw[k] = uint4{x[0], x[1], x[2], x[3]};
+          if constexpr (D != 64) raw[k + G] = uint4{y[0], y[1], y[2], y[3]};
+        }
+      }
+      auto elem = [&](uint32_t w, int hf) -> float {
+        const uint16_t u = (uint16_t)(w >> (16 * hf));
+        return a.q_dtype == DT_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
+      };
+      // the row scaled by 2^e so that its largest |q| lies in [2^14, 2^15)
+      float mx = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 2 * G; ++k)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          mx = fmaxf(mx, fmaxf(fabsf(elem(word_of(raw[k], w), 0)), fabsf(elem(word_of(raw[k], w), 1))));
+      mx = fmaxf(mx, shfl_xor(mx, 16));
+      mx = fmaxf(mx, shfl_xor(mx, 32));
+      const int ex = (int)(__builtin_bit_cast(uint32_t, mx) >> 23);  // biased exponent
+      int up2 = ex == 255 ? 0 : 14 + 127 - ex;
+      up2 = mx > 0.0f ? min(up2, 100) : 0;
+      // (rows past about 2^90 take all their scores some powers of two too small, so
+      // that nothing overflows: scores that differ do so by far more than the
+      // softmax resolves either way)
+      const int es = (int)((__builtin_bit_cast(uint32_t, a.scale_log2) >> 23) & 0xffu) - 127;
+      const int down2 = min(-up2, 100 - es);
+      fr[rt] = ldexpf(a.scale_log2, down2);
+#pragma unroll
+      for (int k = 0; k < 2 * G; ++k) {
+        if ((k & 1) == 0) Z[rt][k >> 1] = 0.0f;
+        half8_t v;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float x0 = ldexpf(elem(word_of(raw[k], w), 0), up2);
+          const float x1 = ldexpf(elem(word_of(raw[k], w), 1), up2);
+          v[2 * w] = rvalid[rt] ? (_Float16)x0 : (_Float16)0.0f;
+          v[2 * w + 1] = rvalid[rt] ? (_Float16)x1 : (_Float16)0.0f;
+          Z[rt][k >> 1] += (float)v[2 * w] + (float)v[2 * w + 1];
+        }
+        qB[rt][k] = v;
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        Z[rt][g] += shfl_xor(Z[rt][g], 16);
+        Z[rt][g] += shfl_xor(Z[rt][g], 32);
+        Z[rt][g] *= fr[rt];
+      }
+    }
+  };
+
+  // ---- the step's new token, where this range holds the sequence's last block:
+  // quantized into LDS, patched into the registers when its block comes up,
+  // stored by row group 0 at the segment's end
+  uint16_t rk[E], rv[E];
+  int patch_i = -1, patch_t = 0;
+  auto owns_new = [&](int bs, int ss) -> bool {
+    if (!a.k_new) return false;
+    const int len = seq_len(bs), nb = seq_blocks_rg(a, len, rg);
+    return nb > 0 && ss + nb <= iend && ((len - 1) >> 6) == nb - 1;
+  };
+  auto load_new = [&](int bs) {
+    const int64_t off = (int64_t)bs * a.kn_sb + (int64_t)hk * a.kn_sh + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      rk[e] = a.k_new[off + e];
+      rv[e] = a.v_new[off + e];
+    }
+  };
+  auto quantize_new = [&](int bs, int ss, auto dtype) {
+    constexpr int DT = decltype(dtype)::value;
+    const int len = seq_len(bs);
+    if (a.rope_cs) rope_row_lanes<D, DT>(rk, rope_row(a, (WIN ? len_of(a, bs) : len) - 1, D));
+    float x[E];
+    uint32_t code[E];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = elem_to_f32<DT>(kv ? rv[e] : rk[e]);
+      const uint32_t meta = q4_quantize_row<D, DT>(x, code);
+#pragma unroll
+      for (int e = 0; e < E; ++e) (kv ? lds.newv : lds.newk)[lane * E + e] = (uint8_t)code[e];
+      if ((lane * E) % 64 == 0) (kv ? lds.newvm : lds.newkm)[lane * E / 64] = meta;
+    }
+    wave_sync();
+    patch_i = ss + seq_blocks_rg(a, len, rg) - 1;
+    patch_t = (len - 1) & 63;
+  };
+  auto prepare_new = [&](int bs, int ss) {
+    if (a.q_dtype == DT_BF16)
+      quantize_new(bs, ss, std::integral_constant<int, DT_BF16>{});
+    else
+      quantize_new(bs, ss, std::integral_constant<int, DT_F16>{});
+  };
+  // the K word of the new token's dims 8 x .. 8 x + 7, and its V byte m
+  auto new_k_word = [&](int x) -> uint32_t {
+    const uint2 c = *reinterpret_cast<const uint2 *>(lds.newk + 8 * x);
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= q4_k_field(((e < 4 ? c.x : c.y) >> (8 * (e & 3))) & 15u, e);
+    return w;
+  };
+  auto new_v_byte = [&](int m) -> uint32_t {
+    const int d = 32 * (m >> 4) + (m & 15);
+    return (uint32_t)lds.newv[d] | ((uint32_t)lds.newv[d + 16] << 4);
+  };
+  auto patch = [&]() {
+    const int t = patch_t;
+    const bool mine = n == (t & 15);
+#pragma unroll
+    for (int tg = 0; tg < 4; ++tg)
+      if ((t >> 4) == tg) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const int p = D == 64 ? tg >> 1 : tg * (D / 128) + (g >> 1);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t w = new_k_word(8 * g + 2 * q4 + h);
+            const int k = (D == 64 ? (tg & 1) : (g & 1)) * 2 + h;
+            set_word(kq[p], k, mine ? w : word_of(kq[p], k));
+          }
+        }
+      }
+    const int slot = q4_v_slot(t);
+    const bool mine_v = q4 == ((t >> 2) & 3);
+    const uint32_t keep = ~(0xffu << (8 * (slot & 3)));
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const uint32_t nv = new_v_byte(16 * p + n) << (8 * (slot & 3));
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        if ((slot >> 2) == w) set_word(vq[p], w, mine_v ? (word_of(vq[p], w) & keep) | nv : word_of(vq[p], w));
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      mk[g] = lane == t ? lds.newkm[g] : mk[g];
+      mv[g] = lane == t ? lds.newvm[g] : mv[g];
+    }
+  };
+  auto store_new = [&](int phys) {
+    uint8_t *reg = head_region(a.lv, phys, hk);
+    for (int x = lane; x < D / 8; x += 64) *reinterpret_cast<uint32_t *>(reg + q4_k_word(D, patch_t, x)) = new_k_word(x);
+    for (int m = lane; m < D / 2; m += 64) reg[q4_v_byte(D, patch_t, m)] = (uint8_t)new_v_byte(m);
+    if (lane < G) {
+      *reinterpret_cast<uint32_t *>(reg + q4_km_offset(D) + (patch_t * G + lane) * 4) = lds.newkm[lane];
+      *reinterpret_cast<uint32_t *>(reg + q4_vm_offset(D) + (patch_t * G + lane) * 4) = lds.newvm[lane];
+    }
+  };
+
+  bool own = owns_new(b, s);
+  if (own) load_new(b);
+  load_q(b);
+  {
+    const __amdgpu_buffer_rsrc_t r = rsrc_of(i0);
+    load_k(r);
+    load_v(r);
+  }
+  if (own) prepare_new(b, s);
+
+  int i = i0;
+  while (true) {
+    const int len = seq_len(b);
+    const int e = s + seq_blocks_rg(a, len, rg);
+    const int seg_end = __builtin_amdgcn_readfirstlane(min(e, iend));
+    int lim[NRT], lo[NRT], wst = 0, lo_hi = 0;
+#pragma unroll
+    for (int rt = 0; rt < NRT; ++rt) {
+      const int r = rbase + 16 * rt + n;
+      lim[rt] = rvalid[rt] ? key_limit(a, len, r / a.R) : 0;
+      lo[rt] = 0;
+    }
+    const int lim_lo = key_limit(a, len, rbase / a.R);  // keys seen by the wave's first row
+    if constexpr (WIN) {
+      wst = win_view_start(a, b);
+#pragma unroll
+      for (int rt = 0; rt < NRT; ++rt) lo[rt] = max(wst, len - a.Lq + (rbase + 16 * rt + n) / a.R - a.window + 1);
+      const int rlast = min(a.NR, rbase + RR) - 1;
+      lo_hi = max(wst, len - a.Lq + rlast / a.R - a.window + 1);
+    }
+    float m_run[NRT], nm[NRT], l_part[NRT], c_part[NRT][G];
+    float4_t o[NRT][NDT];
+#pragma unroll
+    for (int rt = 0; rt < NRT; ++rt) {
+      m_run[rt] = -INFINITY;
+      nm[rt] = 0.0f;
+      l_part[rt] = 0.0f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) c_part[rt][g] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) o[rt][dt] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    int new_phys = -1;
+
+    for (; i < seg_end; ++i) {
+      const int tbase = (i - s) << 6;
+      if (i == patch_i) {
+        patch();
+        new_phys = __builtin_amdgcn_readlane(tab, __builtin_amdgcn_readfirstlane((i - tab0) & 63));
+      }
+      // ---- metadata to LDS
+      bool data = tbase + lane < len;
+      if constexpr (WIN) data = data && tbase + lane >= wst;
+      bool large = false;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        lds.km[64 * g + lane] = mk[g];
+        const uint32_t w = data ? mv[g] : 0u;
+        lds.vm[64 * g + lane] = w;
+        large |= fabsf(lo_f32(w)) > kBig;
+      }
+      const bool big = __any(large);
+      wave_sync();
+
+      // ---- S^T tiles of 16 tokens: lane holds tokens 16 tg + 4 q4 + x of row n,
+      // relative to the running reference
+      float4_t sc[4][NRT];
+#pragma unroll
+      for (int tg = 0; tg < 4; ++tg) {
+        float4_t t[NRT];
+#pragma unroll
+        for (int rt = 0; rt < NRT; ++rt) sc[tg][rt] = float4_t{nm[rt], nm[rt], nm[rt], nm[rt]};
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint4 mw = *reinterpret_cast<const uint4 *>(lds.km + 64 * g + 16 * tg + 4 * q4);
+          float4_t acc[NRT];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 &piece = kq[D == 64 ? tg >> 1 : tg * (D / 128) + (g >> 1)];
+            const half8_t A = q4_k_operand(word_of(piece, (D == 64 ? (tg & 1) : (g & 1)) * 2 + h));
+#pragma unroll
+            for (int rt = 0; rt < NRT; ++rt)
+              acc[rt] = mfma16x16x32(A, qB[rt][2 * g + h], h == 0 ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : acc[rt]);
+          }
+#pragma unroll
+          for (int rt = 0; rt < NRT; ++rt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float sk = lo_f32(word_of(mw, x));
+              t[rt][x] = g == 0 ? sk * acc[rt][x] : __builtin_fmaf(sk, acc[rt][x], t[rt][x]);
+              const float z = __builtin_fmaf(-16.0f, sk, hi_f32(word_of(mw, x)));  // (once for all row tiles)
+              sc[tg][rt][x] = __builtin_fmaf(z, Z[rt][g], sc[tg][rt][x]);
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < NRT; ++rt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sc[tg][rt][x] = __builtin_fmaf(fr[rt], t[rt][x], sc[tg][rt][x]);
+      }
+      if (i + 1 < iend && i + 1 - tab0 == 64) load_table(i + 1);
+      const __amdgpu_buffer_rsrc_t rn = rsrc_of(i + 1);
+      load_k(rn);
+
+      bool edge = tbase + 64 > lim_lo;
+      if constexpr (WIN) edge = edge || tbase < lo_hi;
+      if (edge) {
+#pragma unroll
+        for (int tg = 0; tg < 4; ++tg)
+#pragma unroll
+          for (int rt = 0; rt < NRT; ++rt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int tok = tbase + 16 * tg + 4 * q4 + x;
+              if (tok >= lim[rt] || (WIN && tok < lo[rt])) sc[tg][rt][x] = -INFINITY;
+            }
+      }
+
+      // ---- the reference moves only when some score exceeds it by more than kOver
+      const float over_by = big ? 0.0f : kOver, gap = big ? 0.0f : kGap;
+      float mb[NRT];
+      bool over = false;
+#pragma unroll
+      for (int rt = 0; rt < NRT; ++rt) {
+        float v = fmaxf(sc[0][rt][0], sc[0][rt][1]);
+#pragma unroll
+        for (int k = 2; k < 16; k += 2) v = fmaxf(fmaxf(v, sc[k / 4][rt][k % 4]), sc[k / 4][rt][k % 4 + 1]);
+        mb[rt] = v;
+        over |= v > (m_run[rt] == -INFINITY ? -INFINITY : over_by);
+      }
+      if (__any(over)) {
+#pragma unroll
+        for (int rt = 0; rt < NRT; ++rt) {
+          const float v = swap32_max(swap16_max(mb[rt]));  // the row's, over its four lanes
+          const float mu = m_run[rt] == -INFINITY ? 0.0f : m_run[rt];
+          const float mn = fmaxf(m_run[rt], v + mu - gap);
+          const float al = m_run[rt] == -INFINITY ? 0.0f : fast_exp2(m_run[rt] - mn);
+          const float dn = mn == -INFINITY ? 0.0f : mn - mu;
+#pragma unroll
+          for (int tg = 0; tg < 4; ++tg)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float y = sc[tg][rt][x] - dn;
+              sc[tg][rt][x] = y > gap ? gap : y;  // (keeps a NaN)
+            }
+          m_run[rt] = mn;
+          nm[rt] = mn == -INFINITY ? 0.0f : -mn;
+          l_part[rt] *= al;
+#pragma unroll
+          for (int g = 0; g < G; ++g) c_part[rt][g] *= al;
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) o[rt][dt] *= al;
+        }
+      }
+#pragma unroll
+      for (int rt = 0; rt < NRT; ++rt) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int tg = 0; tg < 4; ++tg)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            sc[tg][rt][x] = fast_exp2(sc[tg][rt][x]);
+            sum += sc[tg][rt][x];
+          }
+        l_part[rt] += sum;
+      }
+
+      // ---- O^T += V^T . P^T: contraction slot 8 q4 + k is token 32 ks + 4 q4 + k
+      // (k < 4) or 32 ks + 16 + 4 q4 + k - 4
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint32_t *vp = lds.vm + 64 * g + 32 * ks + 4 * q4;
+          const uint4 vw[2] = {*reinterpret_cast<const uint4 *>(vp), *reinterpret_cast<const uint4 *>(vp + 16)};
+          half8_t Bh[NRT], Bl[NRT];
+#pragma unroll
+          for (int rt = 0; rt < NRT; ++rt) {
+            float w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t m = word_of(vw[k >> 2], k & 3);
+              const float p = sc[2 * ks + (k >> 2)][rt][k & 3];
+              w[k] = p * lo_f32(m);
+              c_part[rt][g] = __builtin_fmaf(p, hi_f32(m), c_part[rt][g]);
+              c_part[rt][g] = __builtin_fmaf(8.0f, w[k], c_part[rt][g]);
+            }
+            split_hi_lo(float4{w[0], w[1], w[2], w[3]}, float4{w[4], w[5], w[6], w[7]}, Bh[rt], Bl[rt]);
+          }
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {
+            const int j = 2 * g + jj;
+            half8_t Al, Ah;
+            q4_v_operands(word_of(vq[j], 2 * ks), word_of(vq[j], 2 * ks + 1), Al, Ah);
+#pragma unroll
+            for (int rt = 0; rt < NRT; ++rt) {
+              o[rt][2 * j] = mfma16x16x32(Al, Bh[rt], o[rt][2 * j]);
+              o[rt][2 * j + 1] = mfma16x16x32(Ah, Bh[rt], o[rt][2 * j + 1]);
+              o[rt][2 * j] = mfma16x16x32(Al, Bl[rt], o[rt][2 * j]);
+              o[rt][2 * j + 1] = mfma16x16x32(Ah, Bl[rt], o[rt][2 * j + 1]);
+            }
+          }
+        }
+      }
+      load_v(rn);
+      wave_sync();  // (the metadata is read before the next block's is written)
+    }
+
+    // ---- the segment's end: lane holds O^T[16 dt + 4 q4 + x][row n], odd tiles
+    // times 16; output or a partial in slot
+    // (hk row_groups + rg) (waves + B) + range + b
+    const bool whole = !a.partial_only && s >= i0 && e <= iend;
+    const int64_t slot = ((int64_t)hk * a.row_groups + rg) * (a.waves + a.B) + wv + b;
+#pragma unroll
+    for (int rt = 0; rt < NRT; ++rt) {
+      float l = l_part[rt];
+      l += shfl_xor(l, 16);
+      l += shfl_xor(l, 32);
+      float cg[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float c = c_part[rt][g];
+        c += shfl_xor(c, 16);
+        c += shfl_xor(c, 32);
+        cg[g] = c;
+      }
+      if (!rvalid[rt]) continue;
+      const float mul = !whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+      const int64_t pi = slot * RR + 16 * rt + n;
+      const int64_t ob = (whole ? out_row_base(a, b, hk, rbase + 16 * rt + n, D) : pi * D) + 4 * q4;
+      auto put = [&](void *out, auto dtype) {
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) {
+          float run[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            run[x] = ((dt & 1) ? __builtin_fmaf(o[rt][dt][x], 0.0625f, cg[dt / 4]) : o[rt][dt][x] + cg[dt / 4]) * mul;
+          store_run<4>(out, ob + 16 * dt, run, decltype(dtype)::value);
+        }
+      };
+      if (!whole)
+        put(a.ws_o, std::integral_constant<int, DT_F32>{});
+      else if (a.out_dtype == DT_F32)
+        put(a.out, std::integral_constant<int, DT_F32>{});
+      else if (a.out_dtype == DT_F16)
+        put(a.out, std::integral_constant<int, DT_F16>{});
+      else
+        put(a.out, std::integral_constant<int, DT_BF16>{});
+      if (!whole && q4 == 0) reinterpret_cast<float2 *>(a.ws_ml)[pi] = float2{m_run[rt], l};
+    }
+    if (rg == 0 && new_phys >= 0) store_new(new_phys);
+    if (i >= iend) break;
+    // the next sequence with blocks (the merge clears the others' rows)
+    ++b;
+    s = e;
+    while (b < a.B && seq_blocks_rg(a, seq_len(b), rg) == 0) ++b;
+    if (b >= a.B) break;
+    own = owns_new(b, s);
+    if (own) load_new(b);
+    load_q(b);
+    if (own) prepare_new(b, s);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host launchers
+// ---------------------------------------------------------------------------
+namespace {
+
+template <int D, int NRT>
+hipError_t launch_q4(const AttnArgs &args, dim3 grid, hipStream_t st) {
+  if (args.window > 0)
+    k_attn_q4<D, NRT, true><<<grid, dim3(64), 0, st>>>(args);
+  else
+    k_attn_q4<D, NRT, false><<<grid, dim3(64), 0, st>>>(args);
+  return hipGetLastError();
+}
+
+template <int D, int NRT>
+int32_t q4_occupancy() {
+  static const int32_t n = [] {
+    int blocks = 0;
+    const auto *fn = reinterpret_cast<const void *>(&k_attn_q4<D, NRT, false>);
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, fn, 64, 0) != hipSuccess || blocks < 1) {
+      (void)hipGetLastError();
+      blocks = 4 * q4_waves<D, NRT>();
+    }
+    return (int32_t)std::min(blocks, 8 * 4);
+  }();
+  return n;
+}
+
+}  // namespace
+
+// Row tiles per wave: two (each unpacked operand feeds two products) where the
+// registers take them.
+int32_t q4_row_tiles(const PoolGeometry &g, int32_t NR) { return NR > 16 && g.D <= 128 ? 2 : 1; }
+
+int32_t q4_waves_per_cu(const PoolGeometry &g, int32_t nrt) {
+  if (!g.base) return g.D * nrt >= 512 ? 4 : 8;
+  switch (g.D) {
+    case 64: return nrt == 2 ? q4_occupancy<64, 2>() : q4_occupancy<64, 1>();
+    case 128: return nrt == 2 ? q4_occupancy<128, 2>() : q4_occupancy<128, 1>();
+    case 256: return q4_occupancy<256, 1>();
+    default: return q4_occupancy<512, 1>();
+  }
+}
+
+hipError_t launch_attn_q4(const PoolGeometry &g, int32_t layer, const AttnLaunch &a, const AttnPlan &p, hipStream_t st) {
+  if (p.waves < 1 || p.group_waves != 1 || p.rows_per_group != 16 * p.nrt ||
+      (int64_t)p.row_groups * p.rows_per_group < p.NR || (a.k_new && a.Lq != 1) || g.Hkv > 65535 || p.row_groups > 65535)
+    return hipErrorInvalidValue;
+  const AttnArgs args = make_attn_args(g, layer, a, p);
+  const dim3 grid((unsigned)p.waves, (unsigned)g.Hkv, (unsigned)p.row_groups);
+  switch (4 * g.D + p.nrt) {
+    case 4 * 64 + 1: return launch_q4<64, 1>(args, grid, st);
+    case 4 * 64 + 2: return launch_q4<64, 2>(args, grid, st);
+    case 4 * 128 + 1: return launch_q4<128, 1>(args, grid, st);
+    case 4 * 128 + 2: return launch_q4<128, 2>(args, grid, st);
+    case 4 * 256 + 1: return launch_q4<256, 1>(args, grid, st);
+    case 4 * 512 + 1: return launch_q4<512, 1>(args, grid, st);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace krill

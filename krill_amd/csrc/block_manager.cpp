@@ -52,9 +52,9 @@ BlockManager::BlockManager(const BlockManagerConfig &cfg) : cfg_(cfg) {
 }
 
 int64_t BlockManager::memory_bytes(int64_t n) const {
-  // int8 payload for K and V, plus scale and zero for K and V in fp16
+  // the codes of K and V (a byte each, or half of one), plus scale and zero for K and V in fp16
   // (QuantizedKVCache.swift:33-42; G groups per row in affine mode).
-  int64_t kv = 2 * n * cfg_.num_kv_heads * cfg_.head_dim;
+  int64_t kv = 2 * n * cfg_.num_kv_heads * cfg_.head_dim * cfg_.code_bits / 8;
   int64_t meta = 4 * n * cfg_.num_kv_heads * cfg_.groups * 2;
   return kv + meta;
 }

@@ -30,6 +30,7 @@ struct BlockManagerConfig {
   int32_t num_kv_heads = 1;
   int32_t head_dim = 64;
   int32_t groups = 1;             // scale/zero pairs per (token, head)
+  int32_t code_bits = 8;          // bits of a stored element
   int32_t dtype_tag = 2;          // prefix-key dtype tag (2 = int8, PrefixCache.swift:488)
   float watermark = 0.9f;         // occupancy that triggers entry eviction
   int32_t max_entries = 8;        // PrefixCache maxMemoryEntries default (PrefixCache.swift:100)

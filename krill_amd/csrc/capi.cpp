@@ -13,6 +13,7 @@
 #include "block_manager.hpp"
 #include "common.hpp"
 #include "kdev.hpp"
+#include "kdev4.hpp"
 #include "launch.hpp"
 #include "scratch.hpp"
 
@@ -137,7 +138,8 @@ int32_t krill_pool_create(const krill_pool_desc *desc, krill_stream_t stream, kr
     if (d.head_dim != 64 && d.head_dim != 128 && d.head_dim != 256 && d.head_dim != kMaxHeadDim)
       return fail(KRILL_E_UNSUPPORTED, "head_dim %d (supported: 64, 128, 256, 512)", d.head_dim);
     if (d.block_tokens != 64) return fail(KRILL_E_UNSUPPORTED, "block_tokens %d (supported: 64)", d.block_tokens);
-    if (d.quant_mode != KRILL_QUANT_REF_ROW && d.quant_mode != KRILL_QUANT_AFFINE_G64)
+    if (d.quant_mode != KRILL_QUANT_REF_ROW && d.quant_mode != KRILL_QUANT_AFFINE_G64 &&
+        d.quant_mode != KRILL_QUANT_AFFINE4_G64)
       return fail(KRILL_E_INVAL, "quant_mode %d", d.quant_mode);
     if (d.in_dtype != KRILL_DTYPE_F16 && d.in_dtype != KRILL_DTYPE_BF16)
       return fail(KRILL_E_INVAL, "in_dtype %d (bf16 or f16)", d.in_dtype);
@@ -158,10 +160,12 @@ int32_t krill_pool_create(const krill_pool_desc *desc, krill_stream_t stream, kr
     g.num_blocks = d.num_blocks;
     g.Hkv = d.num_kv_heads;
     g.D = d.head_dim;
-    g.G = d.quant_mode == KRILL_QUANT_AFFINE_G64 ? d.head_dim / 64 : 1;
-    g.mode = d.quant_mode == KRILL_QUANT_AFFINE_G64 ? krill::MODE_AFFINE : krill::MODE_REF;
+    g.G = d.quant_mode == KRILL_QUANT_REF_ROW ? 1 : d.head_dim / 64;
+    g.mode = d.quant_mode == KRILL_QUANT_AFFINE4_G64  ? krill::MODE_AFFINE4
+             : d.quant_mode == KRILL_QUANT_AFFINE_G64 ? krill::MODE_AFFINE
+                                                      : krill::MODE_REF;
     g.in_dtype = d.in_dtype == KRILL_DTYPE_BF16 ? krill::DT_BF16 : krill::DT_F16;
-    g.head_bytes = krill::head_region_bytes(g.D, g.G);
+    g.head_bytes = g.mode == krill::MODE_AFFINE4 ? krill::q4_region_bytes(g.D) : krill::head_region_bytes(g.D, g.G);
     g.block_stride = static_cast<int64_t>(g.Hkv) * g.head_bytes;
     g.layer_stride = static_cast<int64_t>(g.num_blocks) * g.block_stride;
     const int64_t total = g.layer_stride * g.num_layers;
@@ -196,6 +200,7 @@ int32_t krill_pool_create(const krill_pool_desc *desc, krill_stream_t stream, kr
     c.num_kv_heads = d.num_kv_heads;
     c.head_dim = d.head_dim;
     c.groups = g.G;
+    c.code_bits = g.mode == krill::MODE_AFFINE4 ? 4 : 8;
     c.watermark = p->desc.evict_watermark;
     c.max_entries = p->desc.max_prefix_entries;
     c.min_prefix_len = p->desc.min_prefix_len;
@@ -511,6 +516,9 @@ int32_t krill_gather(krill_pool_t pool, int32_t layer, const int32_t *dev_block_
   return krill::guarded([&]() -> int32_t {
     krill::clear_error();
     if (int32_t rc = check_device_pool(pool, layer)) return rc;
+    if (pool->geom.mode == krill::MODE_AFFINE4)
+      return fail(KRILL_E_UNSUPPORTED, "snapshots hold a byte per element: a 4-bit pool is read with "
+                  "krill_gather_dequant or krill_read_slots");
     if (B < 0 || S_out < 0 || max_blocks < 0) return fail(KRILL_E_INVAL, "negative B, S_out or max_blocks");
     if (B == 0 || S_out == 0) return KRILL_OK;
     if (!out || !out->keys || !out->values || !out->key_scales || !out->key_zeros || !out->value_scales ||
@@ -546,12 +554,31 @@ int32_t krill_gather_dequant(krill_pool_t pool, int32_t layer, const int32_t *de
   });
 }
 
+int32_t krill_read_slots(krill_pool_t pool, int32_t layer, const int32_t *dev_slot_mapping, int32_t B, int32_t L,
+                         void *dev_k_out, void *dev_v_out, krill_stream_t stream) {
+  return krill::guarded([&]() -> int32_t {
+    krill::clear_error();
+    if (int32_t rc = check_device_pool(pool, layer)) return rc;
+    if (B < 0 || L < 0) return fail(KRILL_E_INVAL, "negative B or L");
+    if (B == 0 || L == 0) return KRILL_OK;
+    if (!dev_k_out || !dev_v_out || !dev_slot_mapping) return fail(KRILL_E_INVAL, "NULL device pointer");
+    DeviceGuard dg(pool->device);
+    hipStream_t st = pick_stream(pool, stream);
+    if (int32_t rc = flush_pending(pool, st)) return rc;
+    hipError_t e = krill::launch_read_slots(pool->geom, layer, dev_slot_mapping, B, L, dev_k_out, dev_v_out, st);
+    if (e != hipSuccess) return hip_fail(e, "read-back of slots launch");
+    return KRILL_OK;
+  });
+}
+
 int32_t krill_scatter(krill_pool_t pool, int32_t layer, const krill_snapshot *in, int32_t B, int32_t S_in,
                       const int32_t *dev_src_start, const int32_t *dev_slot_mapping, int32_t L,
                       krill_stream_t stream) {
   return krill::guarded([&]() -> int32_t {
     krill::clear_error();
     if (int32_t rc = check_device_pool(pool, layer)) return rc;
+    if (pool->geom.mode == krill::MODE_AFFINE4)
+      return fail(KRILL_E_UNSUPPORTED, "snapshots hold a byte per element: a 4-bit pool takes none");
     if (B < 0 || S_in < 0 || L < 0) return fail(KRILL_E_INVAL, "negative B, S_in or L");
     if (B == 0 || L == 0) return KRILL_OK;
     if (!in || !in->keys || !in->values || !in->key_scales || !in->key_zeros || !in->value_scales ||
@@ -940,11 +967,11 @@ static int32_t run_windowed(krill_pool_t pool, int32_t layer, const void *dev_q,
   if (nt.k && plan.use_mfma)
     return fail(KRILL_E_UNSUPPORTED, "the fused windowed step runs on the decode kernel: at most 8 query rows per "
                 "KV head (call krill_quantize_append, then krill_attention_windowed)");
-  if (nt.rope_cs && pool->geom.D > 256)
+  if (nt.rope_cs && pool->geom.D > 256 && !plan.q4)
     return fail(KRILL_E_UNSUPPORTED, "windowed RoPE step at head_dim %d (at most 256)", pool->geom.D);
   const int64_t view = std::min<int64_t>(max_seq_len, (int64_t)Lq + window + 62);
-  if (!plan.use_mfma && pool->geom.D <= 256) {
-    // the decode kernel's per-sequence workgroups: at most 64 blocks per wave
+  if (!plan.use_mfma && !plan.q4 && pool->geom.D <= 256) {
+    // the int8 decode kernel's per-sequence workgroups: at most 64 blocks per wave
     const int32_t lim = krill::valu_window_limit(pool->geom, plan.NR, nt.rope_cs != nullptr);
     if (view > lim)
       return fail(KRILL_E_UNSUPPORTED, "window of %d tokens: the windowed decode kernel reads at most %d tokens per "

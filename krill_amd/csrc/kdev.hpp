@@ -12,7 +12,7 @@ typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 
 enum { DT_F16 = 0, DT_BF16 = 1, DT_F32 = 2 };
-enum { MODE_REF = 0, MODE_AFFINE = 1 };
+enum { MODE_REF = 0, MODE_AFFINE = 1, MODE_AFFINE4 = 2 };  // (4 bits: layout in kdev4.hpp)
 
 constexpr int kBlockTokens = 64;
 

@@ -1,0 +1,131 @@
+// The 4-bit storage mode (affine groups of 64): layout of a block's head
+// region, the quantizer's scalar steps and the conversion of codes into matrix
+// operands.
+#pragma once
+
+#include "kdev.hpp"
+
+namespace krill {
+
+// A (layer, block, KV head) region, D = head_dim, G = D / 64:
+//   [0, 32 D)              K codes: D/32 pieces of 64 x 16 bytes (below)
+//   [32 D, 64 D)           V codes: D/32 pieces of 64 x 16 bytes
+//   [64 D, +256 G)         K (scale, bias) fp16 pairs, (t G + g) 4
+//   [64 D + 256 G, +256 G) V (scale, bias) fp16 pairs
+// Lane l of a wave loads the 16 bytes at 16 l of a piece, so every load of a
+// block is one contiguous KB and arrives as a v_mfma_f32_16x16x32_f16 operand
+// (row l % 16, contraction slots 8 (l / 16) .. +7):
+//  * K: a 32-bit word holds 8 dims of a token.  Lane (n, q) = (l % 16, l / 16)
+//    has words (g, h): dims 64 g + 16 q + 8 h .. +7 of token 16 tg + n.  The
+//    four words of a piece are (g, h) of two groups (head_dim 64: of two 16-token
+//    groups).  Dims 2 a, 2 a + 1 of a word sit where the word, shifted left by 0,
+//    4, -4 or rotated left by 8 for a = 0 .. 3, has bits 6-9 and 22-25: the top
+//    of two fp16 significands.
+//  * V: a byte holds dims d (low nibble) and d + 16 of one token, so a token's
+//    bytes are its own and tokens are written without read-modify-write.  Lane
+//    (n, q) of piece j has 16 tokens of dims 32 j + n and 32 j + 16 + n: tokens
+//    32 ks + 16 a + 4 q + x, x < 4, in word 2 ks + a, byte (x >> 1) + 2 (x & 1):
+//    masks of every other byte leave the order in which the scores' tiles leave
+//    P.
+__host__ __device__ constexpr int q4_region_bytes(int D) { return 64 * D + 512 * (D / 64); }
+__host__ __device__ constexpr int q4_v_offset(int D) { return 32 * D; }
+__host__ __device__ constexpr int q4_km_offset(int D) { return 64 * D; }
+__host__ __device__ constexpr int q4_vm_offset(int D) { return 64 * D + 256 * (D / 64); }
+// byte of the K word of dims 8 x .. 8 x + 7 of token t
+__host__ __device__ constexpr int q4_k_word(int D, int t, int x) {
+  const int g = x >> 3, q = (x >> 1) & 3, h = x & 1, n = t & 15, tg = t >> 4;
+  const int piece = D == 64 ? tg >> 1 : tg * (D / 128) + (g >> 1);
+  const int word = (D == 64 ? (tg & 1) : (g & 1)) * 2 + h;
+  return (piece * 64 + q * 16 + n) * 16 + word * 4;
+}
+// word with pair a of its dims moved to bits 6-9 and 22-25, and the word that such
+// a pair comes from
+__host__ __device__ constexpr uint32_t q4_pair(uint32_t w, int a) {
+  return a == 0 ? w : a == 1 ? w << 4 : a == 2 ? w >> 4 : (w << 8) | (w >> 24);
+}
+__host__ __device__ constexpr uint32_t q4_unpair(uint32_t f, int a) {
+  return a == 0 ? f : a == 1 ? f >> 4 : a == 2 ? f << 4 : (f >> 8) | (f << 24);
+}
+__host__ __device__ constexpr uint32_t q4_k_code(uint32_t w, int e) { return (q4_pair(w, e >> 1) >> (6 + 16 * (e & 1))) & 15u; }
+__host__ __device__ constexpr uint32_t q4_k_field(uint32_t c, int e) { return q4_unpair(c << (6 + 16 * (e & 1)), e >> 1); }
+// byte, inside a lane's 16 of a V piece, of token t
+__host__ __device__ constexpr int q4_v_slot(int t) {
+  return ((t >> 5) & 1) * 8 + ((t >> 4) & 1) * 4 + ((t & 3) >> 1) + 2 * (t & 1);
+}
+// byte of V dims d and d + 16 (d % 32 < 16) of token t; m = 16 (d / 32) + d % 16
+__host__ __device__ constexpr int q4_v_byte(int D, int t, int m) {
+  return q4_v_offset(D) + (((m >> 4) * 64 + ((t >> 2) & 3) * 16 + (m & 15)) << 4) + q4_v_slot(t);
+}
+
+// ---------------------------------------------------------------- quantizer
+// Elements are limited to the fp16 range; per group of 64
+//   b = f16(min w),  s = f16(max(0, (max w - b) / 15)),
+//   c = min(15, rint((w - b) / s)), 0 where s = 0:
+// the codes refer to the scale and bias as they are stored, so the stored
+// values err by half a step (the bias by its own rounding, 2^-11 of it).  A
+// NaN makes its group's scale and bias NaN.
+template <int DT>
+__device__ __forceinline__ float q4_limit(float x) {
+  // (fp16: the infinities; v_med3 would turn a NaN into a number)
+  return x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
+}
+// lo / hi: the group's extremes, nan: whether it holds a NaN
+__device__ __forceinline__ uint32_t q4_params(float lo, float hi, bool nan, float &s, float &b) {
+  const uint16_t bb = f32_to_f16_bits(lo + 0.0f);  // (a minimum of -0 is stored as +0)
+  b = f16_bits_to_f32(bb);
+  const float d = hi - b;
+  const uint16_t sb = f32_to_f16_bits((d > 0.0f ? d : 0.0f) / 15.0f);
+  s = f16_bits_to_f32(sb);
+  return nan ? 0x7e007e00u : (uint32_t)sb | ((uint32_t)bb << 16);
+}
+// r = v_rcp_f32(s): the product with r gives the code of the division (to
+// within one unit) except near a rounding tie, where the division decides:
+// |fl(a r) - a / s| <= 2^-22 |a / s| < 2^-17 for quotients up to 32, and both
+// round alike where a r lies more than 2^-16 from the tie.
+__device__ __forceinline__ uint32_t q4_code(float w, float s, float b, float r) {
+  const float a = w - b;
+  float y = a * r;
+  if (!(fabsf(y) < 32.0f && fabsf(__builtin_amdgcn_fractf(y) - 0.5f) > 0x1p-16f)) y = a / s;
+  y = rintf(y);
+  y = y > 0.0f ? y : 0.0f;  // (s = 0: 0/0, inf and NaN)
+  y = y < 15.0f ? y : 15.0f;
+  return s > 0.0f ? (uint32_t)y : 0u;
+}
+// The value a code stands for, as the caches are read back: fp16, within its
+// range.
+__device__ __forceinline__ uint32_t q4_value_bits(uint32_t c, float s, float b) {
+  const float x = __builtin_fmaf((float)c, s, b);  // (the product is exact)
+  return f32_to_f16_bits(x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x);
+}
+
+// ----------------------------------------------------------- matrix operands
+// Codes become fp16 numbers of their own exponent (a subnormal 2^-24 c would be
+// exact as well, but the matrix instructions align their sums to the operands'
+// exponent fields: with subnormal operands a sum over 2000 tokens was off by 1e-4
+// of the result, so by 2e-7).
+
+// The eight codes of a K word in dim order, as 16 + c: one mask-and-or per pair,
+// three shifts.  (The 16 is in the bias: s c + b = s (16 + c) + (b - 16 s).)
+__device__ __forceinline__ half8_t q4_k_operand(uint32_t w) {
+  constexpr uint32_t m = 0x03c003c0u, one = 0x4c004c00u;
+  return __builtin_bit_cast(half8_t, uint4{(w & m) | one, (q4_pair(w, 1) & m) | one, (q4_pair(w, 2) & m) | one,
+                                           (q4_pair(w, 3) & m) | one});
+}
+// Two codes in the low nibbles of a word's halves as c - 8, in the second nibbles
+// as 16 (c - 8): the sums over tokens need centred codes, or they outgrow the
+// result they leave.
+__device__ __forceinline__ uint32_t q4_centred_lo(uint32_t w) {
+  return h2_as_u32(u32_as_h2((w & 0x000f000fu) | 0x64006400u) + half2_t{(_Float16)-1032.0f, (_Float16)-1032.0f});
+}
+__device__ __forceinline__ uint32_t q4_centred_hi(uint32_t w) {
+  return h2_as_u32(u32_as_h2((w & 0x00f000f0u) | 0x64006400u) + half2_t{(_Float16)-1152.0f, (_Float16)-1152.0f});
+}
+// The eight tokens' codes of two V words: low nibbles (tile 2 j) and second
+// nibbles (tile 2 j + 1, times 16).
+__device__ __forceinline__ void q4_v_operands(uint32_t w0, uint32_t w1, half8_t &lo, half8_t &hi) {
+  const uint32_t u0 = w0 >> 8, u1 = w1 >> 8;
+  lo = __builtin_bit_cast(half8_t, uint4{q4_centred_lo(w0), q4_centred_lo(u0), q4_centred_lo(w1), q4_centred_lo(u1)});
+  hi = __builtin_bit_cast(half8_t, uint4{q4_centred_hi(w0), q4_centred_hi(u0), q4_centred_hi(w1), q4_centred_hi(u1)});
+}
+
+}  // namespace krill

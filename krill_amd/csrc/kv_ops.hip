@@ -550,6 +550,38 @@ __global__ __launch_bounds__(256) void k_gather_dequant(LayerView lv, const int3
   }
 }
 
+// Read-back of slots: row l of (b, h) from slots[b][l], zeros where it names
+// none of the pool's; the values of k_gather_dequant.  A lane per 16 dims of a
+// row (the 4-bit pools' form, and what tiles through LDS: kv_q4.hip).
+template <int D, int G, int MODE>
+__global__ __launch_bounds__(256) void k_read_slots(LayerView lv, const int32_t *__restrict__ slots, int32_t L,
+                                                    int32_t H, int64_t n, uint16_t *k_out, uint16_t *v_out) {
+  constexpr int CH = D / 16, DG = D / G;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int c = (int)(i % CH);
+  const int64_t row = i / CH, bh = row / L;
+  const int h = (int)(bh % H);
+  const int slot = slots[(bh / H) * L + row % L];
+  uint16_t *kd = k_out + row * D + 16 * c, *vd = v_out + row * D + 16 * c;
+  if (slot < 0 || (slot >> 6) >= lv.num_blocks) {
+    const uint4 zero4 = {0u, 0u, 0u, 0u};
+    reinterpret_cast<uint4 *>(kd)[0] = reinterpret_cast<uint4 *>(kd)[1] = zero4;
+    reinterpret_cast<uint4 *>(vd)[0] = reinterpret_cast<uint4 *>(vd)[1] = zero4;
+    return;
+  }
+  const int t = slot & 63, g = (16 * c) / DG;
+  const uint8_t *reg = head_region(lv, slot >> 6, h);
+  uint8_t kq[16], vq[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    kq[e] = reg[k_byte(t, 16 * c + e)];
+    vq[e] = reg[v_byte(D, t, 16 * c + e)];
+  }
+  dequant16<D, G, MODE>(kq, *reinterpret_cast<const uint32_t *>(reg + km_offset(D) + ((t * G + g) << 2)), kd);
+  dequant16<D, G, MODE>(vq, *reinterpret_cast<const uint32_t *>(reg + vm_offset(D, G) + ((t * G + g) << 2)), vd);
+}
+
 // ---------------------------------------------------------------------------
 // Scatter: snapshot rows [src_start[b], +L) -> slots[b][0..L).  Inverse of the
 // gather; restoreQuantized (QuantizedKVCache.swift:122-129) and the int8
@@ -1028,6 +1060,8 @@ hipError_t launch_quantize_append(const PoolGeometry &g, int32_t layer, const vo
                                   int64_t sb, int64_t sh, int64_t sl, const int32_t *slots, int32_t B,
                                   int32_t L, hipStream_t st, const int32_t *rope_pos, const float *rope_cs,
                                   int32_t rope_max_pos) {
+  if (g.mode == MODE_AFFINE4)
+    return launch_q4_append(g, layer, k, v, sb, sh, sl, slots, B, L, st, rope_pos, rope_cs, rope_max_pos);
   const RopeArgs rope{rope_pos, rope_cs, rope_max_pos};
   return rope_pos ? launch_append_rope<true>(g, layer, k, v, sb, sh, sl, slots, B, L, rope, st)
                   : launch_append_rope<false>(g, layer, k, v, sb, sh, sl, slots, B, L, rope, st);
@@ -1036,6 +1070,7 @@ hipError_t launch_quantize_append(const PoolGeometry &g, int32_t layer, const vo
 hipError_t launch_gather(const PoolGeometry &g, int32_t layer, const int32_t *tables, const int32_t *lens,
                          int32_t B, int32_t max_blocks, int32_t S_out, int32_t left_pad, void *keys,
                          void *values, void *ks, void *kz, void *vs, void *vz, hipStream_t st) {
+  if (g.mode == MODE_AFFINE4) return hipErrorInvalidValue;
   if ((int64_t)B * g.Hkv * S_out == 0) return hipSuccess;
   if (B > 65535 || g.Hkv > 65535) return hipErrorInvalidValue;
   const LayerView lv = layer_view(g, layer);
@@ -1060,6 +1095,8 @@ hipError_t launch_gather(const PoolGeometry &g, int32_t layer, const int32_t *ta
 hipError_t launch_gather_dequant(const PoolGeometry &g, int32_t layer, const int32_t *tables,
                                  const int32_t *lens, int32_t B, int32_t max_blocks, int32_t S_out,
                                  int32_t left_pad, void *k_out, void *v_out, hipStream_t st) {
+  if (g.mode == MODE_AFFINE4)
+    return launch_q4_gather_dequant(g, layer, tables, lens, B, max_blocks, S_out, left_pad, k_out, v_out, st);
   if ((int64_t)B * g.Hkv * S_out == 0) return hipSuccess;
   if (B > 65535 || g.Hkv > 65535) return hipErrorInvalidValue;
   const LayerView lv = layer_view(g, layer);
@@ -1077,10 +1114,29 @@ hipError_t launch_gather_dequant(const PoolGeometry &g, int32_t layer, const int
   return hipGetLastError();
 }
 
+hipError_t launch_read_slots(const PoolGeometry &g, int32_t layer, const int32_t *slots, int32_t B, int32_t L,
+                             void *k_out, void *v_out, hipStream_t st) {
+  if (g.mode == MODE_AFFINE4) return launch_q4_read_slots(g, layer, slots, B, L, k_out, v_out, st);
+  const int64_t n = (int64_t)B * g.Hkv * L * (g.D / 16);
+  if (n == 0) return hipSuccess;
+  if ((n + 255) / 256 > INT32_MAX) return hipErrorInvalidValue;
+  const LayerView lv = layer_view(g, layer);
+  const dim3 grid((unsigned)((n + 255) / 256)), block(256);
+  auto *ko = static_cast<uint16_t *>(k_out), *vo = static_cast<uint16_t *>(v_out);
+  KRILL_DISPATCH_D(g.D, {
+    if (g.mode == MODE_REF)
+      k_read_slots<D, 1, MODE_REF><<<grid, block, 0, st>>>(lv, slots, L, g.Hkv, n, ko, vo);
+    else
+      k_read_slots<D, D / 64, MODE_AFFINE><<<grid, block, 0, st>>>(lv, slots, L, g.Hkv, n, ko, vo);
+  });
+  return hipGetLastError();
+}
+
 hipError_t launch_scatter(const PoolGeometry &g, int32_t layer, const void *keys, const void *values,
                           const void *ks, const void *kz, const void *vs, const void *vz, int32_t B,
                           int32_t S_in, const int32_t *src_start, const int32_t *slots, int32_t L,
                           hipStream_t st) {
+  if (g.mode == MODE_AFFINE4) return hipErrorInvalidValue;
   if ((int64_t)B * L * g.Hkv == 0) return hipSuccess;
   if (B > 65535 || g.Hkv > 65535) return hipErrorInvalidValue;
   const LayerView lv = layer_view(g, layer);
@@ -1177,7 +1233,8 @@ int32_t plan_attention(const PoolGeometry &g, int32_t B, int32_t Hq, int32_t Lq,
   // 128 dims (the verify kernel's LDS ring would hold 70 KB per stage), the
   // query rows in groups of at most 8 (the largest divisor of NR up to 8),
   // one grid row group each, every group reading all of the cache
-  const bool dsplit = g.D > 256;
+  const bool q4 = g.mode == MODE_AFFINE4;
+  const bool dsplit = g.D > 256 && !q4;
   if (dsplit && path == 2) return -2;
   const int32_t nb_max = std::max(1, (max_seq_len + 63) / 64);
   const int64_t tmax = (int64_t)B * nb_max;
@@ -1186,11 +1243,22 @@ int32_t plan_attention(const PoolGeometry &g, int32_t B, int32_t Hq, int32_t Lq,
   // long enough (a chosen split: always).  At head_dim 512 that is 9 row groups
   // of the VALU kernel: 256 new rows over contexts of 700 to 3000 (2048 rows
   // per KV head) take 145 us against 310 us.
-  p.prefill = p.NR > 64 && (dsplit ? path == 0 && Lq > 1 : path != 1) &&
+  if (q4)  // (a decode step always runs on the kernel that writes its token)
+    p.prefill = Lq > 1 && (path == 2 || (path == 0 && p.NR > 64 &&
+                                         (split_blocks > 0 || long_window_faster(g, B, nb_max, p.NR, cus))));
+  else
+    p.prefill = p.NR > 64 && (dsplit ? path == 0 && Lq > 1 : path != 1) &&
               (split_blocks > 0 || long_window_faster(g, B, nb_max, p.NR, cus));
-  p.use_mfma = p.prefill || (!dsplit && (path == 2 || (path == 0 && p.NR > 8)));
-  if (!p.use_mfma && !dsplit && p.NR > 8) return -2;
-  if (p.use_mfma) {
+  p.q4 = q4 && !p.prefill;
+  p.use_mfma = p.prefill || (!q4 && !dsplit && (path == 2 || (path == 0 && p.NR > 8)));
+  if (!p.use_mfma && !q4 && !dsplit && p.NR > 8) return -2;
+  if (p.q4) {
+    p.nrt = q4_row_tiles(g, p.NR);
+    p.rows_per_group = 16 * p.nrt;
+    p.row_groups = (p.NR + p.rows_per_group - 1) / p.rows_per_group;
+    p.group_waves = 1;
+    p.token_split = 1;
+  } else if (p.use_mfma) {
     // MFMA: 16 query rows per wave (a row group); the row groups of a KV head
     // go to workgroups of up to 4 waves that share one LDS ring, so a block
     // is fetched once per 4 row groups and the smaller register file of a
@@ -1252,6 +1320,8 @@ int32_t plan_attention(const PoolGeometry &g, int32_t B, int32_t Hq, int32_t Lq,
   if (split_blocks > 0) {
     const int64_t pw = std::min(split_blocks, 64);
     waves = (tmax + pw - 1) / pw;
+  } else if (p.q4) {
+    waves = std::max<int64_t>(1, cus * q4_waves_per_cu(g, p.nrt) / ((int64_t)g.Hkv * p.row_groups));
   } else if (p.use_mfma) {
     const int64_t groups = (p.row_groups + p.group_waves - 1) / p.group_waves;
     int64_t per_cu = p.prefill ? prefill_groups_per_cu(g) : mfma_groups_per_cu(g, p.group_waves, p.token_split);
@@ -1267,8 +1337,8 @@ int32_t plan_attention(const PoolGeometry &g, int32_t B, int32_t Hq, int32_t Lq,
   } else {
     waves = std::max<int64_t>(1, cus * valu_waves_per_cu(g, p.NR) / g.Hkv);
   }
-  // (the long-window kernel reloads its table register every 64 blocks)
-  if (!p.prefill) waves = std::max<int64_t>(waves, (tmax + 63) / 64);
+  // (the long-window and the 4-bit kernel reload their table register every 64 blocks)
+  if (!p.prefill && !p.q4) waves = std::max<int64_t>(waves, (tmax + 63) / 64);
   p.split_blocks = split_blocks > 0 ? std::min(split_blocks, 64) : 0;
   p.nb_cap = nb_max;
   p.waves = (int32_t)waves;
@@ -1323,6 +1393,7 @@ static hipError_t launch_append_newest(const PoolGeometry &g, int32_t layer, con
 static hipError_t launch_attn_kernel(const PoolGeometry &g, int32_t layer, const AttnLaunch &a, const AttnPlan &p,
                                      hipStream_t st) {
   if (p.prefill) return launch_attn_prefill(g, layer, a, p, st);
+  if (p.q4) return launch_attn_q4(g, layer, a, p, st);
   return p.use_mfma ? launch_attn_mfma(g, layer, a, p, st) : launch_attn_valu(g, layer, a, p, st);
 }
 
@@ -1355,7 +1426,7 @@ hipError_t launch_attention_windowed(const PoolGeometry &g, int32_t layer, const
   // kernel's window variants (the MFMA path has no RoPE of the queries, and
   // its separate append launch reads absolute table columns the windowed
   // plan does not cover)
-  if (a.rope_cs && (!a.k_new || g.D > 256)) return hipErrorInvalidValue;
+  if (a.rope_cs && (!a.k_new || (g.D > 256 && !p.q4))) return hipErrorInvalidValue;
   if (a.k_new && (p.use_mfma || a.Lq != 1)) return hipErrorInvalidValue;
   AttnLaunch w = a;
   w.win_start = starts;
@@ -1383,7 +1454,7 @@ hipError_t launch_attention_windowed(const PoolGeometry &g, int32_t layer, const
 // dims, 2 rows, batch of 4: flat 22.6 against 20.2 us at 450 tokens, 23.2 against
 // 25.6 at 767; 128 dims, 8 rows: 19.2 against 20.4 at 767).
 static bool per_sequence_decode(const PoolGeometry &g, const AttnLaunch &a, const AttnPlan &p) {
-  if (p.use_mfma || g.D > 256 || p.split_blocks > 0) return false;
+  if (p.use_mfma || p.q4 || g.D > 256 || p.split_blocks > 0) return false;
   if (a.window > 0 || a.partial_only || a.len_const >= 0 || !a.causal) return false;
   if (a.rope_cs && (!a.k_new || a.Lq != 1)) return false;
   if ((int64_t)a.B * g.Hkv > g.num_cus) return false;
@@ -1408,7 +1479,7 @@ hipError_t launch_attention(const PoolGeometry &g, int32_t layer, const AttnLaun
   hipError_t e = launch_attn_kernel(g, layer, a, p, st);
   if (e != hipSuccess) return e;
   // windowed decode kernel at head_dim <= 256: merged inside its workgroups
-  if (!p.use_mfma && a.window > 0 && g.D <= 256) return hipSuccess;
+  if (!p.use_mfma && !p.q4 && a.window > 0 && g.D <= 256) return hipSuccess;
   return launch_attn_merge(g, layer, a, p, st);
 }
 

@@ -12,7 +12,7 @@ struct PoolGeometry {
   int64_t block_stride = 0;   // bytes per block (all heads)
   int32_t head_bytes = 0;     // bytes per (block, head)
   int32_t num_layers = 0, num_blocks = 0, Hkv = 0, D = 0, G = 1;
-  int32_t mode = 0;           // MODE_REF / MODE_AFFINE
+  int32_t mode = 0;           // MODE_REF / MODE_AFFINE / MODE_AFFINE4
   int32_t in_dtype = 1;       // DT_F16 / DT_BF16
   int32_t num_cus = 0;        // compute units of the pool's device (0: host-only pool)
 };
@@ -65,6 +65,7 @@ struct AttnPlan {
   int32_t token_split;    // MFMA: 2 = one row group per workgroup, its two waves split each block's tokens; else 1
   size_t ws_bytes;
   int32_t prefill;        // 1: the long-window kernel of attn_prefill.hip
+  int32_t q4;             // 1: the kernel of attn_q4.hip (4-bit pools, unless prefill); nrt row tiles per wave
 };
 
 int32_t plan_attention(const PoolGeometry &g, int32_t B, int32_t Hq, int32_t Lq, int32_t max_seq_len,
@@ -82,6 +83,18 @@ hipError_t launch_gather(const PoolGeometry &g, int32_t layer, const int32_t *ta
 hipError_t launch_gather_dequant(const PoolGeometry &g, int32_t layer, const int32_t *tables,
                                  const int32_t *lens, int32_t B, int32_t max_blocks, int32_t S_out,
                                  int32_t left_pad, void *k_out, void *v_out, hipStream_t st);
+// 4-bit pools: the append, the read-back of sequences and of slots (fp16 K/V
+// [B][H][L][D], zeros where a slot names none of the pool's).
+hipError_t launch_q4_append(const PoolGeometry &g, int32_t layer, const void *k, const void *v, int64_t sb, int64_t sh,
+                            int64_t sl, const int32_t *slots, int32_t B, int32_t L, hipStream_t st,
+                            const int32_t *rope_pos, const float *rope_cs, int32_t rope_max_pos);
+hipError_t launch_q4_gather_dequant(const PoolGeometry &g, int32_t layer, const int32_t *tables, const int32_t *lens,
+                                    int32_t B, int32_t max_blocks, int32_t S_out, int32_t left_pad, void *k_out,
+                                    void *v_out, hipStream_t st);
+hipError_t launch_q4_read_slots(const PoolGeometry &g, int32_t layer, const int32_t *slots, int32_t B, int32_t L,
+                                void *k_out, void *v_out, hipStream_t st);
+hipError_t launch_read_slots(const PoolGeometry &g, int32_t layer, const int32_t *slots, int32_t B, int32_t L,
+                             void *k_out, void *v_out, hipStream_t st);
 hipError_t launch_scatter(const PoolGeometry &g, int32_t layer, const void *keys, const void *values,
                           const void *ks, const void *kz, const void *vs, const void *vz, int32_t B,
                           int32_t S_in, const int32_t *src_start, const int32_t *slots, int32_t L,
@@ -118,6 +131,10 @@ int32_t mfma_groups_per_cu(const PoolGeometry &g, int32_t group_waves, int32_t t
 // Resident workgroups (four waves) per compute unit of the long-window kernel.
 int32_t prefill_groups_per_cu(const PoolGeometry &g);
 
+// 16-row tiles per wave and resident waves per compute unit of the 4-bit pools' kernel.
+int32_t q4_row_tiles(const PoolGeometry &g, int32_t NR);
+int32_t q4_waves_per_cu(const PoolGeometry &g, int32_t nrt);
+
 // Per-wave timestamps of the last decode launch (diagnostic build only).
 int32_t wave_stamps(unsigned long long *host, int32_t max_waves);
 
@@ -128,6 +145,8 @@ hipError_t launch_attn_mfma(const PoolGeometry &g, int32_t layer, const AttnLaun
                             hipStream_t st);
 hipError_t launch_attn_prefill(const PoolGeometry &g, int32_t layer, const AttnLaunch &a, const AttnPlan &p,
                                hipStream_t st);
+hipError_t launch_attn_q4(const PoolGeometry &g, int32_t layer, const AttnLaunch &a, const AttnPlan &p,
+                          hipStream_t st);
 hipError_t launch_attn_merge(const PoolGeometry &g, int32_t layer, const AttnLaunch &a, const AttnPlan &p,
                              hipStream_t st);
 

@@ -11,7 +11,7 @@ import numpy as np
 
 from . import _lib as L
 
-QUANT_MODES = {"ref_row": L.QUANT_REF_ROW, "affine_g64": L.QUANT_AFFINE_G64}
+QUANT_MODES = {"ref_row": L.QUANT_REF_ROW, "affine_g64": L.QUANT_AFFINE_G64, "affine4_g64": L.QUANT_AFFINE4_G64}
 
 
 def _torch():
@@ -49,13 +49,15 @@ def _enc(s):
 
 
 class KVPool:
-    """Paged int8 KV pool: `num_blocks` 64-token blocks for every layer and KV head.
+    """Paged int8 or 4-bit KV pool: `num_blocks` 64-token blocks for every layer and KV head.
 
     quant_mode "ref_row" stores the reference's per-(token, head) min/max rows
     (QuantizedKVCache.swift:181-197); "affine_g64" stores affine 8-bit groups
-    of 64 with fp16 scale/bias.  in_dtype is the dtype of the K/V/Q tensors
-    handed to the kernels (bf16 or f16).  host_only pools run the block
-    manager without device memory (kernels are refused).
+    of 64 with fp16 scale/bias; "affine4_g64" 4-bit groups of 64, about half
+    the bytes (no snapshots: gather and scatter are refused).  in_dtype is
+    the dtype of the K/V/Q tensors handed to the kernels (bf16 or f16).
+    host_only pools run the block manager without device memory (kernels
+    are refused).
     """
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_blocks: int,
@@ -69,7 +71,8 @@ class KVPool:
         self.quant_mode = quant_mode
         self.mode = QUANT_MODES[quant_mode]
         self.in_dtype_code = _dtype_code(in_dtype)
-        self.groups = head_dim // 64 if self.mode == L.QUANT_AFFINE_G64 else 1
+        self.groups = 1 if self.mode == L.QUANT_REF_ROW else head_dim // 64
+        self.code_bits = 4 if self.mode == L.QUANT_AFFINE4_G64 else 8
         self.host_only = host_only
         desc = L.PoolDesc(num_layers, num_kv_heads, head_dim, 64, num_blocks, self.mode,
                           self.in_dtype_code, L.POOL_HOST_ONLY if host_only else 0,
@@ -317,6 +320,21 @@ class KVPool:
         L.check(L.lib().krill_gather_dequant(self._h, layer, tables.data_ptr(), lens.data_ptr(), B, mb, S_out,
                                              1 if left_pad else 0, k.data_ptr(), v.data_ptr(),
                                              self._stream(stream)))
+        return k, v
+
+    def read_slots(self, layer: int, slot_mapping, stream=None):
+        """What the cache holds at slot_mapping (int32 [B, L] device): fp16 K and V
+        [B, Hkv, L, D], zeros for slots < 0 (krill_read_slots)."""
+        torch = _torch()
+        self._check_dev("slot_mapping", slot_mapping, torch.int32)
+        if slot_mapping.dim() != 2:
+            raise ValueError("slot_mapping must be [B, L]")
+        B, Lq = slot_mapping.shape
+        shape = (B, self.num_kv_heads, Lq, self.head_dim)
+        k = torch.empty(shape, dtype=torch.float16, device=slot_mapping.device)
+        v = torch.empty(shape, dtype=torch.float16, device=slot_mapping.device)
+        L.check(L.lib().krill_read_slots(self._h, layer, slot_mapping.data_ptr(), B, Lq, k.data_ptr(), v.data_ptr(),
+                                         self._stream(stream)))
         return k, v
 
     def scatter(self, layer: int, snap: dict, src_start, slot_mapping, stream=None):
