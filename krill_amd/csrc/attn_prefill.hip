@@ -464,6 +464,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
         // the layout's words are operands: eight dims of a token (K), eight tokens
         // of two dims (V)
         const int nn = ln & 15, qq = ln >> 4;
+        const uint32_t magic = q4_magic();
 #pragma unroll
         for (int k = 0; k < KP; ++k) {
           const int piece = wid + W * k;
@@ -474,14 +475,14 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
               const int tg = D == 64 ? 2 * piece + (w >> 1) : piece / (D / 128);
               const int g = D == 64 ? 0 : 2 * (piece % (D / 128)) + (w >> 1);
               *reinterpret_cast<half8_t *>(lds.k + (16 * tg + nn) * KTS + (64 * g + 16 * qq + 8 * (w & 1)) * 2) =
-                  q4_k_operand(w4[w]);
+                  q4_k_operand(w4[w], magic);
             }
           } else {
             uint8_t *o = lds.v + (32 * (piece - D / 32) + nn) * VTS + 16 * qq;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
               half8_t lo, hi;
-              q4_v_operands(w4[2 * ks], w4[2 * ks + 1], lo, hi);
+              q4_v_operands(w4[2 * ks], w4[2 * ks + 1], magic, lo, hi);
               *reinterpret_cast<half8_t *>(o + 64 * ks) = lo;
               *reinterpret_cast<half8_t *>(o + 16 * VTS + 64 * ks) = hi;
             }
@@ -508,8 +509,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
           const int mm = m & (64 * G - 1), t = mm / G, g = mm % G;
           const _Float16 sh = __builtin_bit_cast(_Float16, (uint16_t)(mraw[k] & 0xffffu));
           const float sf = (float)sh, zr = f16_bits_to_f32((uint16_t)(mraw[k] >> 16));
-          // (4 bits: K's operands are 16 + c, V's c - 8)
-          const float zf = fmaf(!Q4 ? 128.0f : m < 64 * G ? -16.0f : 8.0f, sf, zr);
+          const float zf = fmaf(Q4 ? 8.0f : 128.0f, sf, zr);
           if (m < 64 * G) {
             lds.ks[g * 64 + t] = sf * a.scale_log2;
             lds.kz[g * 64 + t] = zf * a.scale_log2;
@@ -823,11 +823,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
         for (int dt = 0; dt < NDT; ++dt) {
           float run[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            // (4 bits: odd tiles' codes came times 16)
-            const float o = Q4 && (dt & 1) ? oacc[rt][dt][x] * 0.0625f : oacc[rt][dt][x];
-            run[x] = (o + cg[AFF ? dt / 4 : 0]) * mul;
-          }
+          for (int x = 0; x < 4; ++x) run[x] = (oacc[rt][dt][x] + cg[AFF ? dt / 4 : 0]) * mul;
           store_run<4>(out, ob + 16 * dt, run, decltype(dtype)::value);
         }
       };

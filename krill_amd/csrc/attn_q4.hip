@@ -7,7 +7,7 @@
 //
 // in one pass over the blocks with a running reference m, so a block's bytes go
 // from HBM to registers once and nothing is dequantized:
-//   x = f sum_g s_g (q' . (16 + c))_g + sum_g (b_g - 16 s_g) Z_g,   Z_g = scale log2(e) sum_g q
+//   x = sum_g s'_g (q . (c - 8))_g + sum_g z'_g sum_g q,   s' = s scale log2(e), z' = (b + 8 s) scale log2(e)
 //   o = sum_g [ sum_t (p_t s_tg) (c_t - 8) + sum_t p_t (b_tg + 8 s_tg) ]
 // Codes become matrix operands in one or two instructions per pair, from words
 // loaded in the operands' order (kdev4.hpp): one wave holds 16
@@ -16,10 +16,16 @@
 // rows; the tiles S^T = K . Q^T leave a lane four tokens of one row, which is
 // where O^T += V^T . P^T wants them, so P stays in registers.
 //
-// Numerics: queries are scaled by a power of two per row and held in fp16
-// (exact for bf16 and fp16 inputs down to 2^-25 of the row's largest), sums and
-// the softmax in fp32; a weight p s is split into an fp16 high part and the fp16
-// rounding of the rest (2^-22 of it), two products.
+// Numerics: queries are scaled by a power of two and held in fp16 (exact for bf16
+// and fp16 inputs down to 2^-25 of the row's largest; the power is the wave's,
+// taken into s' and z', unless its rows differ by more than 2^10), sums and the
+// softmax in fp32.  A weight p s enters the product as an fp16 high part and the
+// fp16 rounding of the rest (2^-22 of it); bf16 outputs, whose half step is 2^-9,
+// take the high part alone (2^-12).
+//
+// head_dim above 128: a workgroup of D/128 waves, each 128 dims of K and V (the
+// registers of one wave hold no more); their parts of the scores meet in LDS, one
+// barrier a block, and every wave runs the same softmax on the same sums.
 //
 // Work split: the flat order of the int8 kernels -- per (KV head, row group) the
 // blocks of all sequences end to end, the same number to every wave -- and their
@@ -36,16 +42,42 @@ namespace krill {
 
 namespace {
 
-// Per-wave LDS: the block's metadata words [group][token] (V: zero where the
-// token is not the sequence's), the codes and words of the step's new token.
+// Waves per workgroup, each a slice of the dims.
 template <int D>
+constexpr int q4_slices() { return D > 128 ? D / 128 : 1; }
+
+// LDS of one wave (DW dims, G groups): the block's scales [group][token] (V: zero
+// where the token is not the sequence's; groups of the bias products that do not
+// exist: zero), the codes and words of the step's new token.
+template <int DW>
 struct Q4Lds {
-  static constexpr int G = D / 64;
-  __attribute__((aligned(16))) uint32_t km[64 * G];
-  __attribute__((aligned(16))) uint32_t vm[64 * G];
-  __attribute__((aligned(16))) uint8_t newk[D], newv[D];  // a code per byte
+  static constexpr int G = DW / 64;
+  __attribute__((aligned(16))) float ks[64 * G];  // s'
+  __attribute__((aligned(16))) float kz[64 * 4];  // z'
+  __attribute__((aligned(16))) float vs[64 * G];
+  __attribute__((aligned(16))) float vz[64 * G];  // b + 8 s
+  __attribute__((aligned(16))) uint8_t newk[DW], newv[DW];  // a code per byte
   uint32_t newkm[G], newvm[G];
 };
+
+__device__ __forceinline__ float4_t mfma16x16x4f32(float a, float b, float4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+// Two weights as fp16, and the fp16 rounding of what that leaves; the empty asm
+// keeps the conversions packed and the rest one mixed multiply-add (`one` is 1.0
+// where the compiler cannot see it).
+__device__ __forceinline__ uint32_t round2(float &w0, float &w1) {
+  asm("" : "+v"(w0), "+v"(w1));
+  uint32_t u = h2_as_u32(half2_t{(_Float16)w0, (_Float16)w1});
+  asm("" : "+v"(u));
+  return u;
+}
+__device__ __forceinline__ uint32_t rest2(float w0, float w1, uint32_t h, float one) {
+  const half2_t hh = u32_as_h2(h);
+  float r0 = __builtin_fmaf(w0, one, -(float)hh[0]), r1 = __builtin_fmaf(w1, one, -(float)hh[1]);
+  asm("" : "+v"(r0), "+v"(r1));
+  return h2_as_u32(half2_t{(_Float16)r0, (_Float16)r1});
+}
 
 // LDS of one wave: its operations complete in order, waiting for them orders its
 // lanes' writes before other lanes' reads.
@@ -64,12 +96,8 @@ __device__ __forceinline__ float hi_f32(uint32_t w) { return f16_bits_to_f32((ui
 // the quantizer's scales are below 8740).
 constexpr float kGap = 5.0f, kOver = 8.0f, kBig = 255.0f;
 
-// Waves per SIMD the registers are budgeted for.
-template <int D, int NRT>
-constexpr int q4_waves() { return D * NRT >= 512 ? 1 : 2; }
-
-// One row of K or V (lane: E = D/64 consecutive dims, fp32) as codes: the wave's
-// form of the append kernel's quantizer.
+// One slice of a row of K or V (lane: E = D/64 consecutive dims, fp32) as codes:
+// the wave's form of the append kernel's quantizer.
 template <int D, int DT>
 __device__ __forceinline__ uint32_t q4_quantize_row(const float (&x)[D / 64], uint32_t (&code)[D / 64]) {
   constexpr int E = D / 64, LPG = 64 / E;
@@ -96,17 +124,25 @@ __device__ __forceinline__ uint32_t q4_quantize_row(const float (&x)[D / 64], ui
 
 }  // namespace
 
-// NRT: tiles of 16 query rows per wave.  WIN: sliding window.
-template <int D, int NRT, bool WIN>
-__global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a) {
-  constexpr int G = D / 64;
-  constexpr int NP = D / 32;   // 16-byte pieces per lane of K, and of V
-  constexpr int NDT = D / 16;  // 16-dim tiles of the output
+// NRT: tiles of 16 query rows per wave.  WIN: sliding window.  LOW: the weights'
+// low parts too.
+template <int D, int NRT, bool WIN, bool LOW>
+__global__ __launch_bounds__(64 * q4_slices<D>(), 2) void k_attn_q4(AttnArgs a) {
+  constexpr int DS = q4_slices<D>(), DW = D / DS;
+  constexpr int GD = D / 64;    // groups of a row
+  constexpr int G = DW / 64;    // of the wave's slice
+  constexpr int NP = DW / 32;   // 16-byte pieces per lane of K, and of V
+  constexpr int NDT = DW / 16;  // 16-dim tiles of the output
   constexpr int RR = 16 * NRT;
-  constexpr int E = D / 64;
-  __shared__ Q4Lds<D> lds;
+  constexpr int E = DW / 64;
+  __shared__ Q4Lds<DW> lds_all[DS];
+  // the slices' parts of the scores, two buffers; whether a slice has a large V scale
+  __shared__ __attribute__((aligned(16))) float4_t part[DS > 1 ? 2 : 1][DS][DS > 1 ? 4 * NRT * 64 : 1];
+  __shared__ int part_big[2][DS];
 
   const int lane = threadIdx.x & 63, n = lane & 15, q4 = lane >> 4;
+  const int sl = DS > 1 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) : 0;  // the wave's slice
+  Q4Lds<DW> &lds = lds_all[sl];
   const int hk = blockIdx.y, rg = blockIdx.z;
   // (range w of the heads goes to different XCDs)
   const int wv = (int)((blockIdx.x + (unsigned)hk) % gridDim.x);
@@ -184,149 +220,75 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
   auto ld_words = [](__amdgpu_buffer_rsrc_t r, int off, uint32_t (&w)[G]) {
     if constexpr (G == 1) {
       w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 2);
-    } else if constexpr (G == 2) {
+    } else {
+      static_assert(G == 2, "one or two groups a slice");
       const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 2);
       w[0] = v[0];
       w[1] = v[1];
-    } else {
-#pragma unroll
-      for (int g = 0; g < G; g += 4) {
-        const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * g, 0, 2);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[g + k] = v[k];
-      }
     }
   };
   auto load_k = [&](__amdgpu_buffer_rsrc_t r) {
 #pragma unroll
-    for (int p = 0; p < NP; ++p) kq[p] = ld16(r, p * 1024 + lane * 16);
-    ld_words(r, q4_km_offset(D) + lane * G * 4, mk);
-    ld_words(r, q4_vm_offset(D) + lane * G * 4, mv);
+    // (a slice's pieces: one per 16-token group; head_dim 64: one per two of them)
+    for (int p = 0; p < NP; ++p) kq[p] = ld16(r, (p * DS + sl) * 1024 + lane * 16);
+    ld_words(r, q4_km_offset(D) + (lane * GD + sl * G) * 4, mk);
+    ld_words(r, q4_vm_offset(D) + (lane * GD + sl * G) * 4, mv);
   };
   auto load_v = [&](__amdgpu_buffer_rsrc_t r) {
 #pragma unroll
-    for (int p = 0; p < NP; ++p) vq[p] = ld16(r, q4_v_offset(D) + p * 1024 + lane * 16);
+    for (int p = 0; p < NP; ++p) vq[p] = ld16(r, q4_v_offset(D) + (sl * NP + p) * 1024 + lane * 16);
   };
 
-  // ---- queries of sequence bq: lane (n, q4) holds dims 64 g + 16 q4 + 8 h .. +7
-  // of row n in qB[..][2 g + h]
+  // ---- queries: lane (n, q4) holds dims 64 g + 16 q4 + 8 h .. +7 of the slice of
+  // row n in qB[..][2 g + h]
   half8_t qB[NRT][2 * G];
-  float Z[NRT][G];  // scale log2(e) times the row's sum over group g
-  float fr[NRT];    // what a sum of products takes
+  float qz[NRT];       // the row's sum over group q4 (0 past the groups)
+  float rd[NRT];       // what the row's scores take (1, but where exponents differ)
+  float nmf[NRT];      // and its inverse, which the running reference takes
+  float ksf = 1.0f;    // what s and b of K take
+  bool any_rd = false;
+  float qoff[LOW ? 1 : NRT][G];  // !LOW: what the codes' offsets add to a group's products
   bool rvalid[NRT];
 #pragma unroll
   for (int rt = 0; rt < NRT; ++rt) rvalid[rt] = rbase + 16 * rt + n < a.NR;
-  auto load_q = [&](int bq) {
-#pragma unroll
-    for (int rt = 0; rt < NRT; ++rt) {
-      const int r = rvalid[rt] ? rbase + 16 * rt + n : 0;
-      const int hq = hk * a.R + r % a.R, j = r / a.R;
-      const uint16_t *qp = q_row(a, bq, hq, j) + 16 * q4;
-      uint4 raw[2 * G];
-#pragma unroll
-      for (int k = 0; k < 2 * G; ++k) raw[k] = *reinterpret_cast<const uint4 *>(qp + 64 * (k >> 1) + 8 * (k & 1));
-      if (a.rope_cs) {
-        // dim d < D/2 turns with d + D/2: the same lane's operand G later, or
-        // (head_dim 64) lane ^ 32's
-        const int len = WIN ? len_of(a, bq) : seq_len(bq);  // absolute positions
-        const float *crow = rope_row(a, len - a.Lq + j, D) + (D == 64 ? 16 * (q4 & 1) : 16 * q4);
-#pragma unroll
-        for (int k = 0; k < (D == 64 ? 2 : G); ++k) {
-          uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w}, y[4];
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            y[w] = D == 64 ? (uint32_t)__shfl_xor((int)x[w], 32, 64) : word_of(raw[D == 64 ? 0 : k + G], w);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const float *cp = crow + 64 * (k >> 1) + 8 * (k & 1) + 2 * w;
-            const float2 c2 = *reinterpret_cast<const float2 *>(cp), s2 = *reinterpret_cast<const float2 *>(cp + D / 2);
-            const bool up = D == 64 && q4 >= 2;
-            uint32_t lo = up ? y[w] : x[w], hi = up ? x[w] : y[w];
-            if (a.q_dtype == DT_BF16)
-              rope_pair_words<DT_BF16>(lo, hi, c2, s2);
-            else
-              rope_pair_words<DT_F16>(lo, hi, c2, s2);
-            x[w] = up ? hi : lo;
-            y[w] = up ? lo : hi;
-          }
-          raw[k] = uint4{x[0], x[1], x[2], x[3]};
-          if constexpr (D != 64) raw[k + G] = uint4{y[0], y[1], y[2], y[3]};
-        }
-      }
-      auto elem = [&](uint32_t w, int hf) -> float {
-        const uint16_t u = (uint16_t)(w >> (16 * hf));
-        return a.q_dtype == DT_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
-      };
-      // the row scaled by 2^e so that its largest |q| lies in [2^14, 2^15)
-      float mx = 0.0f;
-#pragma unroll
-      for (int k = 0; k < 2 * G; ++k)
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          mx = fmaxf(mx, fmaxf(fabsf(elem(word_of(raw[k], w), 0)), fabsf(elem(word_of(raw[k], w), 1))));
-      mx = fmaxf(mx, shfl_xor(mx, 16));
-      mx = fmaxf(mx, shfl_xor(mx, 32));
-      const int ex = (int)(__builtin_bit_cast(uint32_t, mx) >> 23);  // biased exponent
-      int up2 = ex == 255 ? 0 : 14 + 127 - ex;
-      up2 = mx > 0.0f ? min(up2, 100) : 0;
-      // (rows past about 2^90 take all their scores some powers of two too small, so
-      // that nothing overflows: scores that differ do so by far more than the
-      // softmax resolves either way)
-      const int es = (int)((__builtin_bit_cast(uint32_t, a.scale_log2) >> 23) & 0xffu) - 127;
-      const int down2 = min(-up2, 100 - es);
-      fr[rt] = ldexpf(a.scale_log2, down2);
-#pragma unroll
-      for (int k = 0; k < 2 * G; ++k) {
-        if ((k & 1) == 0) Z[rt][k >> 1] = 0.0f;
-        half8_t v;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float x0 = ldexpf(elem(word_of(raw[k], w), 0), up2);
-          const float x1 = ldexpf(elem(word_of(raw[k], w), 1), up2);
-          v[2 * w] = rvalid[rt] ? (_Float16)x0 : (_Float16)0.0f;
-          v[2 * w + 1] = rvalid[rt] ? (_Float16)x1 : (_Float16)0.0f;
-          Z[rt][k >> 1] += (float)v[2 * w] + (float)v[2 * w + 1];
-        }
-        qB[rt][k] = v;
-      }
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        Z[rt][g] += shfl_xor(Z[rt][g], 16);
-        Z[rt][g] += shfl_xor(Z[rt][g], 32);
-        Z[rt][g] *= fr[rt];
-      }
-    }
-  };
-
   // ---- the step's new token, where this range holds the sequence's last block:
   // quantized into LDS, patched into the registers when its block comes up,
   // stored by row group 0 at the segment's end
-  uint16_t rk[E], rv[E];
+  uint16_t rk[E], rv[E], rk2[E];  // rk2: the dims that rk's turn with
   int patch_i = -1, patch_t = 0;
   auto owns_new = [&](int bs, int ss) -> bool {
     if (!a.k_new) return false;
     const int len = seq_len(bs), nb = seq_blocks_rg(a, len, rg);
     return nb > 0 && ss + nb <= iend && ((len - 1) >> 6) == nb - 1;
   };
+  const int d0 = sl * DW + lane * E;  // the lane's dims of the new rows
   auto load_new = [&](int bs) {
-    const int64_t off = (int64_t)bs * a.kn_sb + (int64_t)hk * a.kn_sh + lane * E;
+    const int64_t off = (int64_t)bs * a.kn_sb + (int64_t)hk * a.kn_sh;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      rk[e] = a.k_new[off + e];
-      rv[e] = a.v_new[off + e];
+      rk[e] = a.k_new[off + d0 + e];
+      rv[e] = a.v_new[off + d0 + e];
+      if (a.rope_cs) rk2[e] = a.k_new[off + (d0 ^ (D / 2)) + e];
     }
   };
   auto quantize_new = [&](int bs, int ss, auto dtype) {
     constexpr int DT = decltype(dtype)::value;
     const int len = seq_len(bs);
-    if (a.rope_cs) rope_row_lanes<D, DT>(rk, rope_row(a, (WIN ? len_of(a, bs) : len) - 1, D));
     float x[E];
     uint32_t code[E];
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
 #pragma unroll
       for (int e = 0; e < E; ++e) x[e] = elem_to_f32<DT>(kv ? rv[e] : rk[e]);
-      const uint32_t meta = q4_quantize_row<D, DT>(x, code);
+      if (kv == 0 && a.rope_cs) {
+        const float *crow = rope_row(a, (WIN ? len_of(a, bs) : len) - 1, D) + (d0 & (D / 2 - 1));
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float c = crow[e], sn = crow[D / 2 + e], y = elem_to_f32<DT>(rk2[e]);
+          x[e] = round_dt<DT>(d0 >= D / 2 ? y * sn + x[e] * c : x[e] * c - y * sn);
+        }
+      }
+      const uint32_t meta = q4_quantize_row<DW, DT>(x, code);
 #pragma unroll
       for (int e = 0; e < E; ++e) (kv ? lds.newv : lds.newk)[lane * E + e] = (uint8_t)code[e];
       if ((lane * E) % 64 == 0) (kv ? lds.newvm : lds.newkm)[lane * E / 64] = meta;
@@ -341,12 +303,12 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
     else
       quantize_new(bs, ss, std::integral_constant<int, DT_F16>{});
   };
-  // the K word of the new token's dims 8 x .. 8 x + 7, and its V byte m
+  // the K word of the new token's dims 8 x .. 8 x + 7 of the slice, and its V byte m
   auto new_k_word = [&](int x) -> uint32_t {
     const uint2 c = *reinterpret_cast<const uint2 *>(lds.newk + 8 * x);
     uint32_t w = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w |= q4_k_field(((e < 4 ? c.x : c.y) >> (8 * (e & 3))) & 15u, e);
+    for (int e = 0; e < 8; ++e) w |= (((e < 4 ? c.x : c.y) >> (8 * (e & 3))) & 15u) << (4 * q4_nibble(e));
     return w;
   };
   auto new_v_byte = [&](int m) -> uint32_t {
@@ -361,11 +323,11 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
       if ((t >> 4) == tg) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const int p = D == 64 ? tg >> 1 : tg * (D / 128) + (g >> 1);
+          const int p = DW == 64 ? tg >> 1 : tg;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t w = new_k_word(8 * g + 2 * q4 + h);
-            const int k = (D == 64 ? (tg & 1) : (g & 1)) * 2 + h;
+            const int k = (DW == 64 ? (tg & 1) : g) * 2 + h;
             set_word(kq[p], k, mine ? w : word_of(kq[p], k));
           }
         }
@@ -388,26 +350,167 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
   };
   auto store_new = [&](int phys) {
     uint8_t *reg = head_region(a.lv, phys, hk);
-    for (int x = lane; x < D / 8; x += 64) *reinterpret_cast<uint32_t *>(reg + q4_k_word(D, patch_t, x)) = new_k_word(x);
-    for (int m = lane; m < D / 2; m += 64) reg[q4_v_byte(D, patch_t, m)] = (uint8_t)new_v_byte(m);
+    if (lane < DW / 8) *reinterpret_cast<uint32_t *>(reg + q4_k_word(D, patch_t, sl * (DW / 8) + lane)) = new_k_word(lane);
+    if (lane < DW / 2) reg[q4_v_byte(D, patch_t, sl * (DW / 2) + lane)] = (uint8_t)new_v_byte(lane);
     if (lane < G) {
-      *reinterpret_cast<uint32_t *>(reg + q4_km_offset(D) + (patch_t * G + lane) * 4) = lds.newkm[lane];
-      *reinterpret_cast<uint32_t *>(reg + q4_vm_offset(D) + (patch_t * G + lane) * 4) = lds.newvm[lane];
+      const int at = (patch_t * GD + sl * G + lane) * 4;
+      *reinterpret_cast<uint32_t *>(reg + q4_km_offset(D) + at) = lds.newkm[lane];
+      *reinterpret_cast<uint32_t *>(reg + q4_vm_offset(D) + at) = lds.newvm[lane];
     }
   };
 
-  bool own = owns_new(b, s);
-  if (own) load_new(b);
-  load_q(b);
-  {
-    const __amdgpu_buffer_rsrc_t r = rsrc_of(i0);
-    load_k(r);
-    load_v(r);
-  }
-  if (own) prepare_new(b, s);
-
+#pragma unroll
+  for (int g = G; g < 4; ++g) lds.kz[64 * g + lane] = 0.0f;
+  float one = 1.0f;
+  asm volatile("" : "+v"(one));
+  const uint32_t magic = q4_magic();
   int i = i0;
   while (true) {
+    // ---- the segment's queries and new token, ahead of the range's first block
+    const bool own = owns_new(b, s);
+    if (own) load_new(b);
+    // (the row's largest |q| over all slices, the queries the slice's turn with)
+    uint4 raw[NRT][2 * G], raw2[NRT][2 * G];
+    float mxr[NRT], mxw = 0.0f;
+    auto elem = [&](uint32_t w, int hf) -> float {
+      const uint16_t u = (uint16_t)(w >> (16 * hf));
+      return a.q_dtype == DT_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
+    };
+    auto largest = [&](const uint4 &v, float m) -> float {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) m = fmaxf(m, fmaxf(fabsf(elem(word_of(v, w), 0)), fabsf(elem(word_of(v, w), 1))));
+      return m;
+    };
+    auto q_piece = [&](int rt, int slice, int k) -> uint4 {
+      const int r = rvalid[rt] ? rbase + 16 * rt + n : 0;
+      const uint16_t *qp = q_row(a, b, hk * a.R + r % a.R, r / a.R) + slice * DW + 16 * q4;
+      return *reinterpret_cast<const uint4 *>(qp + 64 * (k >> 1) + 8 * (k & 1));
+    };
+    constexpr int HALF = DW == D ? 0 : DS / 2;  // slices to the dims that turn together
+#pragma unroll
+    for (int rt = 0; rt < NRT; ++rt)
+#pragma unroll
+      for (int k = 0; k < 2 * G; ++k) {
+        raw[rt][k] = q_piece(rt, sl, k);
+        raw2[rt][k] = uint4{0u, 0u, 0u, 0u};
+        if (HALF && a.rope_cs) raw2[rt][k] = q_piece(rt, sl ^ HALF, k);
+      }
+    if (i == i0) {
+      const __amdgpu_buffer_rsrc_t r = rsrc_of(i0);
+      load_k(r);
+      load_v(r);
+    }
+    if (own) prepare_new(b, s);
+#pragma unroll
+    for (int rt = 0; rt < NRT; ++rt) {
+      float mx = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 2 * G; ++k) mx = largest(raw[rt][k], mx);
+      for (int o = 1; o < DS; ++o)
+#pragma unroll
+        for (int k = 0; k < 2 * G; ++k) mx = largest(q_piece(rt, (sl + o) % DS, k), mx);
+      mx = fmaxf(mx, shfl_xor(mx, 16));
+      mx = fmaxf(mx, shfl_xor(mx, 32));
+      mxr[rt] = rvalid[rt] ? mx : 0.0f;
+      mxw = fmaxf(mxw, mxr[rt]);
+      if (a.rope_cs) {
+        // dims d and d + D/2 turn together: in another slice's piece, this lane's
+        // operand (head_dim 128) or lane ^ 32's (64)
+        const int j = (rvalid[rt] ? rbase + 16 * rt + n : 0) / a.R;
+        const int len = WIN ? len_of(a, b) : seq_len(b);  // absolute positions
+        const float *crow = rope_row(a, len - a.Lq + j, D);
+        uint4 old[2 * G];
+#pragma unroll
+        for (int k = 0; k < 2 * G; ++k) old[k] = raw[rt][k];
+#pragma unroll
+        for (int k = 0; k < 2 * G; ++k) {
+          const int d = sl * DW + 64 * (k >> 1) + 16 * q4 + 8 * (k & 1);
+          const bool up = d >= D / 2;
+          const float *cp = crow + (d & (D / 2 - 1));
+          uint32_t x[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t own_w = word_of(old[k], w);
+            const uint32_t other = HALF        ? word_of(raw2[rt][k], w)
+                                   : DW == 128 ? word_of(old[(k + G) % (2 * G)], w)
+                                               : (uint32_t)__shfl_xor((int)own_w, 32, 64);
+            const float2 c2 = *reinterpret_cast<const float2 *>(cp + 2 * w);
+            const float2 s2 = *reinterpret_cast<const float2 *>(cp + D / 2 + 2 * w);
+            uint32_t lo = up ? other : own_w, hi = up ? own_w : other;
+            if (a.q_dtype == DT_BF16)
+              rope_pair_words<DT_BF16>(lo, hi, c2, s2);
+            else
+              rope_pair_words<DT_F16>(lo, hi, c2, s2);
+            x[w] = up ? hi : lo;
+          }
+          raw[rt][k] = uint4{x[0], x[1], x[2], x[3]};
+        }
+      }
+    }
+    // a row whose largest |q| is mx scaled by 2^e has it in [2^14, 2^15) (a turn may
+    // take it a factor sqrt 2 higher: [2^13, 2^14))
+    auto exponent = [&](float mx) -> int {
+      const int ex = (int)(__builtin_bit_cast(uint32_t, mx) >> 23);
+      return mx > 0.0f && ex < 255 ? min((a.rope_cs ? 140 : 141) - ex, 100) : 0;
+    };
+    // (where the wave's largest |q| passes some 2^90 its scores are taken some
+    // powers of two too small, so that nothing overflows: scores that differ do so
+    // by far more than the softmax resolves either way)
+    const int ew = exponent(row_allmax(mxw));
+    const int es = (int)((__builtin_bit_cast(uint32_t, a.scale_log2) >> 23) & 0xffu) - 127;
+    const int cw = min(-ew, 100 - es);
+    ksf = ldexpf(a.scale_log2, cw);
+    bool differ = false;
+#pragma unroll
+    for (int rt = 0; rt < NRT; ++rt) {
+      int er = ew;
+      rd[rt] = nmf[rt] = 1.0f;
+      if (mxr[rt] > 0.0f && exponent(mxr[rt]) > ew + 10) {
+        er = exponent(mxr[rt]);
+        rd[rt] = ldexpf(1.0f, max(-er - cw, -126));
+        nmf[rt] = 1.0f / rd[rt];
+        differ = true;
+      }
+      float qsum[G];
+#pragma unroll
+      for (int k = 0; k < 2 * G; ++k) {
+        if ((k & 1) == 0) qsum[k >> 1] = 0.0f;
+        half8_t v;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float x0 = ldexpf(elem(word_of(raw[rt][k], w), 0), er);
+          const float x1 = ldexpf(elem(word_of(raw[rt][k], w), 1), er);
+          v[2 * w] = rvalid[rt] ? (_Float16)x0 : (_Float16)0.0f;
+          v[2 * w + 1] = rvalid[rt] ? (_Float16)x1 : (_Float16)0.0f;
+          const float sum = (float)v[2 * w] + (float)v[2 * w + 1];
+          qsum[k >> 1] += sum;
+          if constexpr (!LOW) {
+            // (the codes come as 1024 + c and 1024 + 16 c: what is too much is
+            // where the products start from)
+            if (w & 1) {
+              v[2 * w] *= (_Float16)0.0625f;
+              v[2 * w + 1] *= (_Float16)0.0625f;
+            }
+            qoff[rt][k >> 1] = __builtin_fmaf((w & 1) ? -64.0f : -1024.0f, sum, k % 2 == 0 && w == 0 ? 0.0f : qoff[rt][k >> 1]);
+          }
+        }
+        qB[rt][k] = v;
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        qsum[g] += shfl_xor(qsum[g], 16);
+        qsum[g] += shfl_xor(qsum[g], 32);
+        if constexpr (!LOW) {
+          qoff[rt][g] += shfl_xor(qoff[rt][g], 16);
+          qoff[rt][g] += shfl_xor(qoff[rt][g], 32);
+        }
+      }
+      qz[rt] = 0.0f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) qz[rt] = q4 == g ? qsum[g] : qz[rt];
+    }
+    any_rd = __any(differ);
+
     const int len = seq_len(b);
     const int e = s + seq_blocks_rg(a, len, rg);
     const int seg_end = __builtin_amdgcn_readfirstlane(min(e, iend));
@@ -452,12 +555,15 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
       bool large = false;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        lds.km[64 * g + lane] = mk[g];
+        const float ks = lo_f32(mk[g]) * ksf;
+        lds.ks[64 * g + lane] = ks;
+        lds.kz[64 * g + lane] = __builtin_fmaf(hi_f32(mk[g]), ksf, LOW ? 8.0f * ks : 0.0f);
         const uint32_t w = data ? mv[g] : 0u;
-        lds.vm[64 * g + lane] = w;
-        large |= fabsf(lo_f32(w)) > kBig;
+        lds.vs[64 * g + lane] = lo_f32(w);
+        lds.vz[64 * g + lane] = __builtin_fmaf(8.0f, lo_f32(w), hi_f32(w));
+        large |= lo_f32(w) > kBig;
       }
-      const bool big = __any(large);
+      bool big = __any(large);
       wave_sync();
 
       // ---- S^T tiles of 16 tokens: lane holds tokens 16 tg + 4 q4 + x of row n,
@@ -465,35 +571,58 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
       float4_t sc[4][NRT];
 #pragma unroll
       for (int tg = 0; tg < 4; ++tg) {
-        float4_t t[NRT];
 #pragma unroll
-        for (int rt = 0; rt < NRT; ++rt) sc[tg][rt] = float4_t{nm[rt], nm[rt], nm[rt], nm[rt]};
+        for (int rt = 0; rt < NRT; ++rt) {
+          const float st = DS == 1 || sl == 0 ? nm[rt] : 0.0f;
+          sc[tg][rt] = mfma16x16x4f32(lds.kz[64 * q4 + 16 * tg + n], qz[rt], float4_t{st, st, st, st});
+        }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const uint4 mw = *reinterpret_cast<const uint4 *>(lds.km + 64 * g + 16 * tg + 4 * q4);
+          const float4_t ks = *reinterpret_cast<const float4_t *>(lds.ks + 64 * g + 16 * tg + 4 * q4);
           float4_t acc[NRT];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint4 &piece = kq[D == 64 ? tg >> 1 : tg * (D / 128) + (g >> 1)];
-            const half8_t A = q4_k_operand(word_of(piece, (D == 64 ? (tg & 1) : (g & 1)) * 2 + h));
+            const uint32_t w = word_of(kq[DW == 64 ? tg >> 1 : tg], (DW == 64 ? (tg & 1) : g) * 2 + h);
+            const half8_t A = LOW ? q4_k_operand(w, magic) : q4_k_operand_raw(w, magic);
 #pragma unroll
             for (int rt = 0; rt < NRT; ++rt)
-              acc[rt] = mfma16x16x32(A, qB[rt][2 * g + h], h == 0 ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : acc[rt]);
+              {
+                const float st = LOW ? 0.0f : qoff[LOW ? 0 : rt][g];
+                acc[rt] = mfma16x16x32(A, qB[rt][2 * g + h], h == 0 ? float4_t{st, st, st, st} : acc[rt]);
+              }
           }
 #pragma unroll
           for (int rt = 0; rt < NRT; ++rt)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float sk = lo_f32(word_of(mw, x));
-              t[rt][x] = g == 0 ? sk * acc[rt][x] : __builtin_fmaf(sk, acc[rt][x], t[rt][x]);
-              const float z = __builtin_fmaf(-16.0f, sk, hi_f32(word_of(mw, x)));  // (once for all row tiles)
-              sc[tg][rt][x] = __builtin_fmaf(z, Z[rt][g], sc[tg][rt][x]);
-            }
+            for (int x = 0; x < 4; ++x) sc[tg][rt][x] = __builtin_fmaf(ks[x], acc[rt][x], sc[tg][rt][x]);
+        }
+      }
+      if constexpr (DS > 1) {
+        // the slices' parts: every wave adds them in the same order
+        float4_t(*const mine)[DS > 1 ? 4 * NRT * 64 : 1] = part[i & 1];
+#pragma unroll
+        for (int k = 0; k < 4 * NRT; ++k) mine[sl][64 * k + lane] = sc[k / NRT][k % NRT];
+        if (lane == 0) part_big[i & 1][sl] = big;
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < 4 * NRT; ++k) {
+          float4_t v = mine[0][64 * k + lane];
+#pragma unroll
+          for (int o = 1; o < DS; ++o) v += mine[o][64 * k + lane];
+          sc[k / NRT][k % NRT] = v;
         }
 #pragma unroll
-        for (int rt = 0; rt < NRT; ++rt)
+        for (int o = 0; o < DS; ++o) big = big || part_big[i & 1][o] != 0;
+        big = __any(big);
+      }
+      if (any_rd) {
+        asm volatile("; rows of other exponents");  // (a branch, not a multiplication by one)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) sc[tg][rt][x] = __builtin_fmaf(fr[rt], t[rt][x], sc[tg][rt][x]);
+        for (int tg = 0; tg < 4; ++tg)
+#pragma unroll
+          for (int rt = 0; rt < NRT; ++rt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sc[tg][rt][x] *= rd[rt];
       }
       if (i + 1 < iend && i + 1 - tab0 == 64) load_table(i + 1);
       const __amdgpu_buffer_rsrc_t rn = rsrc_of(i + 1);
@@ -541,7 +670,7 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
               sc[tg][rt][x] = y > gap ? gap : y;  // (keeps a NaN)
             }
           m_run[rt] = mn;
-          nm[rt] = mn == -INFINITY ? 0.0f : -mn;
+          nm[rt] = mn == -INFINITY ? 0.0f : -mn * nmf[rt];
           l_part[rt] *= al;
 #pragma unroll
           for (int g = 0; g < G; ++g) c_part[rt][g] *= al;
@@ -568,33 +697,41 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
       for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const uint32_t *vp = lds.vm + 64 * g + 32 * ks + 4 * q4;
-          const uint4 vw[2] = {*reinterpret_cast<const uint4 *>(vp), *reinterpret_cast<const uint4 *>(vp + 16)};
+          const int at = 64 * g + 32 * ks + 4 * q4;
+          const float4_t vs[2] = {*reinterpret_cast<const float4_t *>(lds.vs + at),
+                                  *reinterpret_cast<const float4_t *>(lds.vs + at + 16)};
+          const float4_t vz[2] = {*reinterpret_cast<const float4_t *>(lds.vz + at),
+                                  *reinterpret_cast<const float4_t *>(lds.vz + at + 16)};
           half8_t Bh[NRT], Bl[NRT];
 #pragma unroll
           for (int rt = 0; rt < NRT; ++rt) {
-            float w[8];
+            uint32_t bh[4], bl[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint32_t m = word_of(vw[k >> 2], k & 3);
-              const float p = sc[2 * ks + (k >> 2)][rt][k & 3];
-              w[k] = p * lo_f32(m);
-              c_part[rt][g] = __builtin_fmaf(p, hi_f32(m), c_part[rt][g]);
-              c_part[rt][g] = __builtin_fmaf(8.0f, w[k], c_part[rt][g]);
+            for (int k = 0; k < 8; k += 2) {
+              const float4_t &p = sc[2 * ks + (k >> 2)][rt];
+              const int x = k & 3;
+              c_part[rt][g] = __builtin_fmaf(p[x], vz[k >> 2][x], c_part[rt][g]);
+              c_part[rt][g] = __builtin_fmaf(p[x + 1], vz[k >> 2][x + 1], c_part[rt][g]);
+              float w0 = p[x] * vs[k >> 2][x], w1 = p[x + 1] * vs[k >> 2][x + 1];
+              bh[k / 2] = round2(w0, w1);
+              if constexpr (LOW) bl[k / 2] = rest2(w0, w1, bh[k / 2], one);
             }
-            split_hi_lo(float4{w[0], w[1], w[2], w[3]}, float4{w[4], w[5], w[6], w[7]}, Bh[rt], Bl[rt]);
+            Bh[rt] = __builtin_bit_cast(half8_t, uint4{bh[0], bh[1], bh[2], bh[3]});
+            if constexpr (LOW) Bl[rt] = __builtin_bit_cast(half8_t, uint4{bl[0], bl[1], bl[2], bl[3]});
           }
 #pragma unroll
           for (int jj = 0; jj < 2; ++jj) {
             const int j = 2 * g + jj;
             half8_t Al, Ah;
-            q4_v_operands(word_of(vq[j], 2 * ks), word_of(vq[j], 2 * ks + 1), Al, Ah);
+            q4_v_operands(word_of(vq[j], 2 * ks), word_of(vq[j], 2 * ks + 1), magic, Al, Ah);
 #pragma unroll
             for (int rt = 0; rt < NRT; ++rt) {
               o[rt][2 * j] = mfma16x16x32(Al, Bh[rt], o[rt][2 * j]);
               o[rt][2 * j + 1] = mfma16x16x32(Ah, Bh[rt], o[rt][2 * j + 1]);
-              o[rt][2 * j] = mfma16x16x32(Al, Bl[rt], o[rt][2 * j]);
-              o[rt][2 * j + 1] = mfma16x16x32(Ah, Bl[rt], o[rt][2 * j + 1]);
+              if constexpr (LOW) {
+                o[rt][2 * j] = mfma16x16x32(Al, Bl[rt], o[rt][2 * j]);
+                o[rt][2 * j + 1] = mfma16x16x32(Ah, Bl[rt], o[rt][2 * j + 1]);
+              }
             }
           }
         }
@@ -603,9 +740,8 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
       wave_sync();  // (the metadata is read before the next block's is written)
     }
 
-    // ---- the segment's end: lane holds O^T[16 dt + 4 q4 + x][row n], odd tiles
-    // times 16; output or a partial in slot
-    // (hk row_groups + rg) (waves + B) + range + b
+    // ---- the segment's end: lane holds O^T[16 dt + 4 q4 + x][row n]; output or a
+    // partial in slot (hk row_groups + rg) (waves + B) + range + b
     const bool whole = !a.partial_only && s >= i0 && e <= iend;
     const int64_t slot = ((int64_t)hk * a.row_groups + rg) * (a.waves + a.B) + wv + b;
 #pragma unroll
@@ -624,14 +760,14 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
       if (!rvalid[rt]) continue;
       const float mul = !whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
       const int64_t pi = slot * RR + 16 * rt + n;
-      const int64_t ob = (whole ? out_row_base(a, b, hk, rbase + 16 * rt + n, D) : pi * D) + 4 * q4;
+      const int64_t ob = (whole ? out_row_base(a, b, hk, rbase + 16 * rt + n, D) : pi * D) + sl * DW + 4 * q4;
       auto put = [&](void *out, auto dtype) {
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
           float run[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-            run[x] = ((dt & 1) ? __builtin_fmaf(o[rt][dt][x], 0.0625f, cg[dt / 4]) : o[rt][dt][x] + cg[dt / 4]) * mul;
+            run[x] = (o[rt][dt][x] + cg[dt / 4]) * mul;
           store_run<4>(out, ob + 16 * dt, run, decltype(dtype)::value);
         }
       };
@@ -643,7 +779,7 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
         put(a.out, std::integral_constant<int, DT_F16>{});
       else
         put(a.out, std::integral_constant<int, DT_BF16>{});
-      if (!whole && q4 == 0) reinterpret_cast<float2 *>(a.ws_ml)[pi] = float2{m_run[rt], l};
+      if (!whole && sl == 0 && q4 == 0) reinterpret_cast<float2 *>(a.ws_ml)[pi] = float2{m_run[rt], l};
     }
     if (rg == 0 && new_phys >= 0) store_new(new_phys);
     if (i >= iend) break;
@@ -652,10 +788,6 @@ __global__ __launch_bounds__(64, (q4_waves<D, NRT>())) void k_attn_q4(AttnArgs a
     s = e;
     while (b < a.B && seq_blocks_rg(a, seq_len(b), rg) == 0) ++b;
     if (b >= a.B) break;
-    own = owns_new(b, s);
-    if (own) load_new(b);
-    load_q(b);
-    if (own) prepare_new(b, s);
   }
 }
 
@@ -666,10 +798,19 @@ namespace {
 
 template <int D, int NRT>
 hipError_t launch_q4(const AttnArgs &args, dim3 grid, hipStream_t st) {
-  if (args.window > 0)
-    k_attn_q4<D, NRT, true><<<grid, dim3(64), 0, st>>>(args);
-  else
-    k_attn_q4<D, NRT, false><<<grid, dim3(64), 0, st>>>(args);
+  const bool low = args.out_dtype != DT_BF16;
+  const dim3 block(64 * q4_slices<D>());
+  if (args.window > 0) {
+    if (low)
+      k_attn_q4<D, NRT, true, true><<<grid, block, 0, st>>>(args);
+    else
+      k_attn_q4<D, NRT, true, false><<<grid, block, 0, st>>>(args);
+  } else {
+    if (low)
+      k_attn_q4<D, NRT, false, true><<<grid, block, 0, st>>>(args);
+    else
+      k_attn_q4<D, NRT, false, false><<<grid, block, 0, st>>>(args);
+  }
   return hipGetLastError();
 }
 
@@ -677,29 +818,29 @@ template <int D, int NRT>
 int32_t q4_occupancy() {
   static const int32_t n = [] {
     int blocks = 0;
-    const auto *fn = reinterpret_cast<const void *>(&k_attn_q4<D, NRT, false>);
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, fn, 64, 0) != hipSuccess || blocks < 1) {
+    const auto *fn = reinterpret_cast<const void *>(&k_attn_q4<D, NRT, false, true>);
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, fn, 64 * q4_slices<D>(), 0) != hipSuccess || blocks < 1) {
       (void)hipGetLastError();
-      blocks = 4 * q4_waves<D, NRT>();
+      blocks = 8 / q4_slices<D>();
     }
-    return (int32_t)std::min(blocks, 8 * 4);
+    return (int32_t)blocks;
   }();
   return n;
 }
 
 }  // namespace
 
-// Row tiles per wave: two (each unpacked operand feeds two products) where the
-// registers take them.
-int32_t q4_row_tiles(const PoolGeometry &g, int32_t NR) { return NR > 16 && g.D <= 128 ? 2 : 1; }
+// Row tiles per wave: two from 17 rows on (each unpacked operand feeds two
+// products).
+int32_t q4_row_tiles(int32_t NR) { return NR > 16 ? 2 : 1; }
 
-int32_t q4_waves_per_cu(const PoolGeometry &g, int32_t nrt) {
-  if (!g.base) return g.D * nrt >= 512 ? 4 : 8;
+int32_t q4_groups_per_cu(const PoolGeometry &g, int32_t nrt) {
+  if (!g.base) return g.D <= 128 ? 8 : 8 * 128 / g.D;
   switch (g.D) {
     case 64: return nrt == 2 ? q4_occupancy<64, 2>() : q4_occupancy<64, 1>();
     case 128: return nrt == 2 ? q4_occupancy<128, 2>() : q4_occupancy<128, 1>();
-    case 256: return q4_occupancy<256, 1>();
-    default: return q4_occupancy<512, 1>();
+    case 256: return nrt == 2 ? q4_occupancy<256, 2>() : q4_occupancy<256, 1>();
+    default: return nrt == 2 ? q4_occupancy<512, 2>() : q4_occupancy<512, 1>();
   }
 }
 
@@ -715,7 +856,9 @@ hipError_t launch_attn_q4(const PoolGeometry &g, int32_t layer, const AttnLaunch
     case 4 * 128 + 1: return launch_q4<128, 1>(args, grid, st);
     case 4 * 128 + 2: return launch_q4<128, 2>(args, grid, st);
     case 4 * 256 + 1: return launch_q4<256, 1>(args, grid, st);
+    case 4 * 256 + 2: return launch_q4<256, 2>(args, grid, st);
     case 4 * 512 + 1: return launch_q4<512, 1>(args, grid, st);
+    case 4 * 512 + 2: return launch_q4<512, 2>(args, grid, st);
     default: return hipErrorInvalidValue;
   }
 }

@@ -18,9 +18,9 @@ namespace krill {
 //  * K: a 32-bit word holds 8 dims of a token.  Lane (n, q) = (l % 16, l / 16)
 //    has words (g, h): dims 64 g + 16 q + 8 h .. +7 of token 16 tg + n.  The
 //    four words of a piece are (g, h) of two groups (head_dim 64: of two 16-token
-//    groups).  Dims 2 a, 2 a + 1 of a word sit where the word, shifted left by 0,
-//    4, -4 or rotated left by 8 for a = 0 .. 3, has bits 6-9 and 22-25: the top
-//    of two fp16 significands.
+//    groups).  Dim e of a word sits in nibble (e >> 1) + 4 (e & 1), so that masks
+//    of the low and of the second nibble of both halves, before and after a shift
+//    by 8, leave the pairs (0,1), (2,3), (4,5), (6,7).
 //  * V: a byte holds dims d (low nibble) and d + 16 of one token, so a token's
 //    bytes are its own and tokens are written without read-modify-write.  Lane
 //    (n, q) of piece j has 16 tokens of dims 32 j + n and 32 j + 16 + n: tokens
@@ -38,16 +38,7 @@ __host__ __device__ constexpr int q4_k_word(int D, int t, int x) {
   const int word = (D == 64 ? (tg & 1) : (g & 1)) * 2 + h;
   return (piece * 64 + q * 16 + n) * 16 + word * 4;
 }
-// word with pair a of its dims moved to bits 6-9 and 22-25, and the word that such
-// a pair comes from
-__host__ __device__ constexpr uint32_t q4_pair(uint32_t w, int a) {
-  return a == 0 ? w : a == 1 ? w << 4 : a == 2 ? w >> 4 : (w << 8) | (w >> 24);
-}
-__host__ __device__ constexpr uint32_t q4_unpair(uint32_t f, int a) {
-  return a == 0 ? f : a == 1 ? f >> 4 : a == 2 ? f << 4 : (f >> 8) | (f << 24);
-}
-__host__ __device__ constexpr uint32_t q4_k_code(uint32_t w, int e) { return (q4_pair(w, e >> 1) >> (6 + 16 * (e & 1))) & 15u; }
-__host__ __device__ constexpr uint32_t q4_k_field(uint32_t c, int e) { return q4_unpair(c << (6 + 16 * (e & 1)), e >> 1); }
+__host__ __device__ constexpr int q4_nibble(int e) { return (e >> 1) + 4 * (e & 1); }
 // byte, inside a lane's 16 of a V piece, of token t
 __host__ __device__ constexpr int q4_v_slot(int t) {
   return ((t >> 5) & 1) * 8 + ((t >> 4) & 1) * 4 + ((t & 3) >> 1) + 2 * (t & 1);
@@ -104,28 +95,49 @@ __device__ __forceinline__ uint32_t q4_value_bits(uint32_t c, float s, float b) 
 // exponent fields: with subnormal operands a sum over 2000 tokens was off by 1e-4
 // of the result, so by 2e-7).
 
-// The eight codes of a K word in dim order, as 16 + c: one mask-and-or per pair,
-// three shifts.  (The 16 is in the bias: s c + b = s (16 + c) + (b - 16 s).)
-__device__ __forceinline__ half8_t q4_k_operand(uint32_t w) {
-  constexpr uint32_t m = 0x03c003c0u, one = 0x4c004c00u;
-  return __builtin_bit_cast(half8_t, uint4{(w & m) | one, (q4_pair(w, 1) & m) | one, (q4_pair(w, 2) & m) | one,
-                                           (q4_pair(w, 3) & m) | one});
+// Centred as well, c - 8: sums of codes of one sign outgrow the result they
+// leave.  Two instructions a pair, (1024 + c) - 1032 of the low nibbles of a
+// word's halves, (1024 + 16 c) / 16 - 72 of the second nibbles.  `magic` is
+// q4_magic() in a vector register: v_and_or_b32 takes one scalar operand and no
+// literal (with both constants known to the compiler it becomes two
+// instructions).
+__device__ __forceinline__ uint32_t q4_magic() {
+  uint32_t m;
+  asm("v_mov_b32 %0, 0x64006400" : "=v"(m));
+  return m;
 }
-// Two codes in the low nibbles of a word's halves as c - 8, in the second nibbles
-// as 16 (c - 8): the sums over tokens need centred codes, or they outgrow the
-// result they leave.
-__device__ __forceinline__ uint32_t q4_centred_lo(uint32_t w) {
-  return h2_as_u32(u32_as_h2((w & 0x000f000fu) | 0x64006400u) + half2_t{(_Float16)-1032.0f, (_Float16)-1032.0f});
+__device__ __forceinline__ uint32_t q4_and_or(uint32_t w, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(magic));
+  return r;
 }
-__device__ __forceinline__ uint32_t q4_centred_hi(uint32_t w) {
-  return h2_as_u32(u32_as_h2((w & 0x00f000f0u) | 0x64006400u) + half2_t{(_Float16)-1152.0f, (_Float16)-1152.0f});
+__device__ __forceinline__ uint32_t q4_centred_lo(uint32_t w, uint32_t magic) {
+  return h2_as_u32(u32_as_h2(q4_and_or(w, 0x000f000fu, magic)) + half2_t{(_Float16)-1032.0f, (_Float16)-1032.0f});
 }
-// The eight tokens' codes of two V words: low nibbles (tile 2 j) and second
-// nibbles (tile 2 j + 1, times 16).
-__device__ __forceinline__ void q4_v_operands(uint32_t w0, uint32_t w1, half8_t &lo, half8_t &hi) {
+__device__ __forceinline__ uint32_t q4_centred_hi(uint32_t w, uint32_t magic) {
+  const half2_t r = half2_t{(_Float16)0.0625f, (_Float16)0.0625f}, m = half2_t{(_Float16)-72.0f, (_Float16)-72.0f};
+  return h2_as_u32(__builtin_elementwise_fma(u32_as_h2(q4_and_or(w, 0x00f000f0u, magic)), r, m));
+}
+// The eight codes of a K word in dim order.
+__device__ __forceinline__ half8_t q4_k_operand(uint32_t w, uint32_t magic) {
+  const uint32_t u = w >> 8;
+  return __builtin_bit_cast(half8_t, uint4{q4_centred_lo(w, magic), q4_centred_hi(w, magic), q4_centred_lo(u, magic),
+                                           q4_centred_hi(u, magic)});
+}
+// The same as they come, 1024 + c in pairs 0 and 2, 1024 + 16 c in pairs 1 and 3.
+__device__ __forceinline__ half8_t q4_k_operand_raw(uint32_t w, uint32_t magic) {
+  const uint32_t u = w >> 8;
+  return __builtin_bit_cast(half8_t, uint4{q4_and_or(w, 0x000f000fu, magic), q4_and_or(w, 0x00f000f0u, magic),
+                                           q4_and_or(u, 0x000f000fu, magic), q4_and_or(u, 0x00f000f0u, magic)});
+}
+// The eight tokens' codes of two V words: low nibbles (tile 2 j), second nibbles
+// (tile 2 j + 1).
+__device__ __forceinline__ void q4_v_operands(uint32_t w0, uint32_t w1, uint32_t magic, half8_t &lo, half8_t &hi) {
   const uint32_t u0 = w0 >> 8, u1 = w1 >> 8;
-  lo = __builtin_bit_cast(half8_t, uint4{q4_centred_lo(w0), q4_centred_lo(u0), q4_centred_lo(w1), q4_centred_lo(u1)});
-  hi = __builtin_bit_cast(half8_t, uint4{q4_centred_hi(w0), q4_centred_hi(u0), q4_centred_hi(w1), q4_centred_hi(u1)});
+  lo = __builtin_bit_cast(half8_t, uint4{q4_centred_lo(w0, magic), q4_centred_lo(u0, magic), q4_centred_lo(w1, magic),
+                                         q4_centred_lo(u1, magic)});
+  hi = __builtin_bit_cast(half8_t, uint4{q4_centred_hi(w0, magic), q4_centred_hi(u0, magic), q4_centred_hi(w1, magic),
+                                         q4_centred_hi(u1, magic)});
 }
 
 }  // namespace krill

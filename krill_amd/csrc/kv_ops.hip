@@ -1253,7 +1253,7 @@ int32_t plan_attention(const PoolGeometry &g, int32_t B, int32_t Hq, int32_t Lq,
   p.use_mfma = p.prefill || (!q4 && !dsplit && (path == 2 || (path == 0 && p.NR > 8)));
   if (!p.use_mfma && !q4 && !dsplit && p.NR > 8) return -2;
   if (p.q4) {
-    p.nrt = q4_row_tiles(g, p.NR);
+    p.nrt = q4_row_tiles(p.NR);
     p.rows_per_group = 16 * p.nrt;
     p.row_groups = (p.NR + p.rows_per_group - 1) / p.rows_per_group;
     p.group_waves = 1;
@@ -1321,7 +1321,7 @@ int32_t plan_attention(const PoolGeometry &g, int32_t B, int32_t Hq, int32_t Lq,
     const int64_t pw = std::min(split_blocks, 64);
     waves = (tmax + pw - 1) / pw;
   } else if (p.q4) {
-    waves = std::max<int64_t>(1, cus * q4_waves_per_cu(g, p.nrt) / ((int64_t)g.Hkv * p.row_groups));
+    waves = std::max<int64_t>(1, cus * q4_groups_per_cu(g, p.nrt) / ((int64_t)g.Hkv * p.row_groups));
   } else if (p.use_mfma) {
     const int64_t groups = (p.row_groups + p.group_waves - 1) / p.group_waves;
     int64_t per_cu = p.prefill ? prefill_groups_per_cu(g) : mfma_groups_per_cu(g, p.group_waves, p.token_split);

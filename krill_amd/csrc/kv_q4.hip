@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256) void k_q4_append(LayerView lv, const uint16_t 
         if (kv == 0) {
           uint32_t word = 0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) word |= q4_k_field(code[e], e);
+          for (int e = 0; e < 8; ++e) word |= code[e] << (4 * q4_nibble(e));
           if (r >= 0) *reinterpret_cast<uint32_t *>(im.bytes + q4_k_word(D, r, x)) = word;
         } else {
           // bytes of dims (d, d + 16): the lane's and those of lane x ^ 2, four each
@@ -340,8 +340,8 @@ __global__ __launch_bounds__(256) void k_q4_read(LayerView lv, Q4Read a, uint16_
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-          const uint32_t c0 = kv ? ((e < 4 ? v0 : v1) >> (8 * (e & 3))) & 15u : q4_k_code(kw, e);
-          const uint32_t c1 = kv ? ((e < 4 ? v0 : v1) >> (8 * ((e + 1) & 3))) & 15u : q4_k_code(kw, e + 1);
+          const uint32_t c0 = kv ? ((e < 4 ? v0 : v1) >> (8 * (e & 3))) & 15u : (kw >> (4 * q4_nibble(e))) & 15u;
+          const uint32_t c1 = kv ? ((e < 4 ? v0 : v1) >> (8 * ((e + 1) & 3))) & 15u : (kw >> (4 * q4_nibble(e + 1))) & 15u;
           w[e / 2] = q4_value_bits(c0, s, bias) | (q4_value_bits(c1, s, bias) << 16);
         }
         res[kv] = uint4{w[0], w[1], w[2], w[3]};

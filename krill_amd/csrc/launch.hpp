@@ -131,9 +131,9 @@ int32_t mfma_groups_per_cu(const PoolGeometry &g, int32_t group_waves, int32_t t
 // Resident workgroups (four waves) per compute unit of the long-window kernel.
 int32_t prefill_groups_per_cu(const PoolGeometry &g);
 
-// 16-row tiles per wave and resident waves per compute unit of the 4-bit pools' kernel.
-int32_t q4_row_tiles(const PoolGeometry &g, int32_t NR);
-int32_t q4_waves_per_cu(const PoolGeometry &g, int32_t nrt);
+// 16-row tiles per wave and resident workgroups per compute unit of the 4-bit pools' kernel.
+int32_t q4_row_tiles(int32_t NR);
+int32_t q4_groups_per_cu(const PoolGeometry &g, int32_t nrt);
 
 // Per-wave timestamps of the last decode launch (diagnostic build only).
 int32_t wave_stamps(unsigned long long *host, int32_t max_waves);

@@ -61,16 +61,25 @@ def weight_error(G):
     return (6 * G + 4) * 2.0 ** -24 * 8 + 2.0 ** -19
 
 
-def bound(q, k, v, scale, want, out):
+def bound(q, k, v, scale, want, out, sk=0.0, sv=0.0):
     """Largest error a row of the kernels' output may show, given float64 q [n, D], k, v [T, D].
 
     Queries and codes enter the products exactly, so a score errs by the roundings of its sums: per
     group of 64 dims two matrix steps, the scale's and the bias's multiply-add, and two at the end,
     each at most 2^-23 of the sum of the terms' sizes; a weight 2^x errs by as much relative (times
-    ln 2) and by 2^-22 in the exponential, its split and the sums; the output by half a step."""
+    ln 2) and by 2^-22 in the exponential, its split and the sums; the output by half a step.
+
+    bf16 outputs: weights are rounded to fp16 (2^-11) and weigh |c - 8| s <= 8 sv, sv the largest
+    scale of V; codes of K enter as 1024 + c or 1024 + 16 c (over 16 queries), so a group's three
+    sums of products, from the offset's start to two matrix steps, are at most 2^-23 of 1040 times
+    the group's |q| off, in units of the scale, sk the largest."""
     G = k.shape[-1] // 64
     terms = np.abs(q) @ np.abs(k).max(0) * 2.0  # |s c| and |b| are each at most twice the value's range
     dx = (6 * G + 4) * 2.0 ** -23 * terms * abs(scale) * np.log2(np.e)
+    low = 0.0
+    if out == "bf16":
+        dx = dx + 3 * 2.0 ** -23 * 1040 * np.abs(q).sum(-1) * sk * abs(scale) * np.log2(np.e)
+        low = 2.0 ** -11 * 8 * sv
     vmax = 2.0 * np.abs(v).max()
     rel = 2 * np.log(2.0) * dx + 2.0 ** -19
-    return (rel * vmax)[:, None] + 0.5 * EPS[out] * np.abs(want) + 2.0 ** -25
+    return (rel * vmax)[:, None] + low + 0.5 * EPS[out] * np.abs(want) + 2.0 ** -25

@@ -69,7 +69,8 @@ class Cache:
                 if T == 0:
                     assert not g.any()
                     continue
-                err, lim = np.abs(g - want), Q.bound(rows, kd, vd, scale, want, out)
+                err, lim = np.abs(g - want), Q.bound(rows, kd, vd, scale, want, out, *(
+                    Q.quantize(x[b][h], self.dt)[1].max(initial=0) for x in (self.k, self.v)))
                 assert np.all(err <= lim), f"b {b} h {h}: {np.nanmax(err / lim):.3g} times the bound"
                 # errors of the weights are independent, as the values they weigh: both sum alike
                 x = np.abs(rows @ kd.T).max() * abs(scale) * np.log2(np.e)
