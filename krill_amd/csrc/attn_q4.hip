@@ -96,38 +96,17 @@ __device__ __forceinline__ float hi_f32(uint32_t w) { return f16_bits_to_f32((ui
 // the quantizer's scales are below 8740).
 constexpr float kGap = 5.0f, kOver = 8.0f, kBig = 255.0f;
 
-// One slice of a row of K or V (lane: E = D/64 consecutive dims, fp32) as codes:
-// the wave's form of the append kernel's quantizer.
-template <int D, int DT>
-__device__ __forceinline__ uint32_t q4_quantize_row(const float (&x)[D / 64], uint32_t (&code)[D / 64]) {
-  constexpr int E = D / 64, LPG = 64 / E;
-  float w[E], lo = INFINITY, hi = -INFINITY;
-  bool nan = false;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    nan |= x[e] != x[e];
-    w[e] = q4_limit<DT>(x[e]);
-    lo = fminf(lo, w[e]);
-    hi = fmaxf(hi, w[e]);
-  }
-  lo = wave_min_range<1, LPG / 2>(lo);
-  hi = wave_max_range<1, LPG / 2>(hi);
-  const uint64_t in_group = (LPG == 64 ? ~0ull : ((1ull << (LPG & 63)) - 1)) << ((threadIdx.x & 63) / LPG * LPG);
-  const bool any = (__ballot(nan) & in_group) != 0;
-  float s, b;
-  const uint32_t meta = q4_params(lo, hi, any, s, b);
-  const float r = __builtin_amdgcn_rcpf(s);
-#pragma unroll
-  for (int e = 0; e < E; ++e) code[e] = q4_code(w[e], s, b, r);
-  return meta;
-}
+constexpr int kSeqWaves = 8, kSeqRows = 8;
 
 }  // namespace
 
 // NRT: tiles of 16 query rows per wave.  WIN: sliding window.  LOW: the weights'
-// low parts too.
-template <int D, int NRT, bool WIN, bool LOW>
-__global__ __launch_bounds__(64 * q4_slices<D>(), 2) void k_attn_q4(AttnArgs a) {
+// low parts too.  SEQ: instead of the flat split a workgroup of kSeqWaves waves
+// per (sequence, KV head), each a share of its blocks, their partial results
+// combined in LDS (at most kSeqRows query rows, head_dim up to 128).
+template <int D, int NRT, bool WIN, bool LOW, bool SEQ>
+__global__ __launch_bounds__(64 * (SEQ ? kSeqWaves : q4_slices<D>()), 2) void k_attn_q4(AttnArgs a) {
+  static_assert(!SEQ || (NRT == 1 && D <= 128), "one slice, one row tile");
   constexpr int DS = q4_slices<D>(), DW = D / DS;
   constexpr int GD = D / 64;    // groups of a row
   constexpr int G = DW / 64;    // of the wave's slice
@@ -135,54 +114,68 @@ __global__ __launch_bounds__(64 * q4_slices<D>(), 2) void k_attn_q4(AttnArgs a) 
   constexpr int NDT = DW / 16;  // 16-dim tiles of the output
   constexpr int RR = 16 * NRT;
   constexpr int E = DW / 64;
-  __shared__ Q4Lds<DW> lds_all[DS];
+  __shared__ Q4Lds<DW> lds_all[SEQ ? kSeqWaves : DS];
   // the slices' parts of the scores, two buffers; whether a slice has a large V scale
   __shared__ __attribute__((aligned(16))) float4_t part[DS > 1 ? 2 : 1][DS][DS > 1 ? 4 * NRT * 64 : 1];
   __shared__ int part_big[2][DS];
+  // SEQ: each wave's partial, rows of o (padded by four banks), (m, l)
+  __shared__ __attribute__((aligned(16))) float seq_o[SEQ ? kSeqWaves : 1][SEQ ? kSeqRows * (D + 4) : 4];
+  __shared__ float2 seq_ml[SEQ ? kSeqWaves : 1][kSeqRows];
 
   const int lane = threadIdx.x & 63, n = lane & 15, q4 = lane >> 4;
   const int sl = DS > 1 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) : 0;  // the wave's slice
-  Q4Lds<DW> &lds = lds_all[sl];
+  const int wid = SEQ ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) : 0;
+  Q4Lds<DW> &lds = lds_all[SEQ ? wid : sl];
   const int hk = blockIdx.y, rg = blockIdx.z;
   // (range w of the heads goes to different XCDs)
   const int wv = (int)((blockIdx.x + (unsigned)hk) % gridDim.x);
   const int rbase = rg * RR;
 
   // ---- flat blocks [i0, iend) of the (head, row group) order
-  int c0 = 0, lenv = lane < a.B ? seq_len_view<WIN>(a, lane) : 0;
-  int nbv = seq_blocks_rg(a, lenv, rg);
-  int incl = wave_incl_scan(nbv);
-  int T = __builtin_amdgcn_readlane(incl, 63);
-  for (int cc = 64; cc < a.B; cc += 64) {
-    const int bb = cc + lane;
-    T += __builtin_amdgcn_readfirstlane(wave_allsum_int(bb < a.B ? seq_blocks_rg(a, seq_len_view<WIN>(a, bb), rg) : 0));
-  }
-  // (every wave that takes part holds a block: the merge relies on it)
-  const int Wt = min(a.waves, T);
-  if (wv >= Wt) return;
-  const int i0 = __builtin_amdgcn_readfirstlane((int)(((int64_t)wv * T + Wt - 1) / Wt));
-  const int iend = __builtin_amdgcn_readfirstlane((int)(((int64_t)(wv + 1) * T + Wt - 1) / Wt));
+  int c0 = 0, lenv = 0, i0 = 0, iend = 0;
   int b = -1, s = 0;  // the sequence of block i0, the flat index of its first block
-  {
-    int carry = 0;
-    for (c0 = 0; c0 < a.B; c0 += 64) {
-      if (c0 > 0) {
-        const int bb = c0 + lane;
-        lenv = bb < a.B ? seq_len_view<WIN>(a, bb) : 0;
-        nbv = seq_blocks_rg(a, lenv, rg);
-        incl = wave_incl_scan(nbv) + carry;
-      }
-      const unsigned long long m = __ballot(c0 + lane < a.B && incl > i0);
-      if (m) {
-        const int l = __builtin_ctzll(m);
-        b = c0 + l;
-        s = __builtin_amdgcn_readlane(incl - nbv, l);
-        break;
-      }
-      carry = __builtin_amdgcn_readlane(incl, 63);
+  if constexpr (SEQ) {
+    // (blocks counted from the sequence's first)
+    b = c0 = (int)blockIdx.x;
+    lenv = seq_len_view<WIN>(a, b);
+    const int nb = seq_blocks_rg(a, lenv, rg);
+    i0 = (wid * nb + kSeqWaves - 1) / kSeqWaves;
+    iend = ((wid + 1) * nb + kSeqWaves - 1) / kSeqWaves;
+  } else {
+    lenv = lane < a.B ? seq_len_view<WIN>(a, lane) : 0;
+    int nbv = seq_blocks_rg(a, lenv, rg);
+    int incl = wave_incl_scan(nbv);
+    int T = __builtin_amdgcn_readlane(incl, 63);
+    for (int cc = 64; cc < a.B; cc += 64) {
+      const int bb = cc + lane;
+      T += __builtin_amdgcn_readfirstlane(wave_allsum_int(bb < a.B ? seq_blocks_rg(a, seq_len_view<WIN>(a, bb), rg) : 0));
     }
+    // (every wave that takes part holds a block: the merge relies on it)
+    const int Wt = min(a.waves, T);
+    if (wv >= Wt) return;
+    i0 = __builtin_amdgcn_readfirstlane((int)(((int64_t)wv * T + Wt - 1) / Wt));
+    iend = __builtin_amdgcn_readfirstlane((int)(((int64_t)(wv + 1) * T + Wt - 1) / Wt));
+    {
+      int carry = 0;
+      for (c0 = 0; c0 < a.B; c0 += 64) {
+        if (c0 > 0) {
+          const int bb = c0 + lane;
+          lenv = bb < a.B ? seq_len_view<WIN>(a, bb) : 0;
+          nbv = seq_blocks_rg(a, lenv, rg);
+          incl = wave_incl_scan(nbv) + carry;
+        }
+        const unsigned long long m = __ballot(c0 + lane < a.B && incl > i0);
+        if (m) {
+          const int l = __builtin_ctzll(m);
+          b = c0 + l;
+          s = __builtin_amdgcn_readlane(incl - nbv, l);
+          break;
+        }
+        carry = __builtin_amdgcn_readlane(incl, 63);
+      }
+    }
+    if (b < 0) return;
   }
-  if (b < 0) return;
   auto seq_len = [&](int bs) -> int { return bs - c0 < 64 ? __builtin_amdgcn_readlane(lenv, bs - c0) : seq_len_view<WIN>(a, bs); };
 
   // block-table entries of flat blocks tab0 .. tab0 + 63, one a lane (-1: none
@@ -259,7 +252,7 @@ __global__ __launch_bounds__(64 * q4_slices<D>(), 2) void k_attn_q4(AttnArgs a) 
   auto owns_new = [&](int bs, int ss) -> bool {
     if (!a.k_new) return false;
     const int len = seq_len(bs), nb = seq_blocks_rg(a, len, rg);
-    return nb > 0 && ss + nb <= iend && ((len - 1) >> 6) == nb - 1;
+    return nb > 0 && i0 < iend && ss + nb <= iend && ((len - 1) >> 6) == nb - 1;
   };
   const int d0 = sl * DW + lane * E;  // the lane's dims of the new rows
   auto load_new = [&](int bs) {
@@ -365,7 +358,7 @@ __global__ __launch_bounds__(64 * q4_slices<D>(), 2) void k_attn_q4(AttnArgs a) 
   asm volatile("" : "+v"(one));
   const uint32_t magic = q4_magic();
   int i = i0;
-  while (true) {
+  while (!SEQ || i0 < iend) {
     // ---- the segment's queries and new token, ahead of the range's first block
     const bool own = owns_new(b, s);
     if (own) load_new(b);
@@ -743,6 +736,25 @@ __global__ __launch_bounds__(64 * q4_slices<D>(), 2) void k_attn_q4(AttnArgs a) 
     // ---- the segment's end: lane holds O^T[16 dt + 4 q4 + x][row n]; output or a
     // partial in slot (hk row_groups + rg) (waves + B) + range + b
     const bool whole = !a.partial_only && s >= i0 && e <= iend;
+    if constexpr (SEQ) {
+      float l = l_part[0];
+      l += shfl_xor(l, 16);
+      l += shfl_xor(l, 32);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float c = c_part[0][g];
+        c += shfl_xor(c, 16);
+        c += shfl_xor(c, 32);
+        if (n < kSeqRows) {
+#pragma unroll
+          for (int dt = 4 * g; dt < 4 * g + 4; ++dt)
+            *reinterpret_cast<float4_t *>(&seq_o[wid][n * (D + 4) + 16 * dt + 4 * q4]) = o[0][dt] + c;
+        }
+      }
+      if (q4 == 0 && n < kSeqRows) seq_ml[wid][n] = float2{m_run[0], l};
+      if (new_phys >= 0) store_new(new_phys);
+      break;
+    }
     const int64_t slot = ((int64_t)hk * a.row_groups + rg) * (a.waves + a.B) + wv + b;
 #pragma unroll
     for (int rt = 0; rt < NRT; ++rt) {
@@ -789,6 +801,33 @@ __global__ __launch_bounds__(64 * q4_slices<D>(), 2) void k_attn_q4(AttnArgs a) 
     while (b < a.B && seq_blocks_rg(a, seq_len(b), rg) == 0) ++b;
     if (b >= a.B) break;
   }
+
+  if constexpr (SEQ) {
+    // a wave that had no block left nothing behind
+    if (i0 >= iend && lane < kSeqRows) seq_ml[wid][lane] = float2{-INFINITY, 0.0f};
+    __syncthreads();
+    const int b0 = (int)blockIdx.x;
+    const int nrow = min(kSeqRows, a.NR - rbase);
+    for (int t = threadIdx.x; t < nrow * (D / 4); t += 64 * kSeqWaves) {
+      const int r = t / (D / 4), d = 4 * (t % (D / 4));
+      float M = -INFINITY, L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kSeqWaves; ++w) M = fmaxf(M, seq_ml[w][r].x);
+      float4_t acc = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < kSeqWaves; ++w) {
+        const float2 ml = seq_ml[w][r];
+        // (a row whose scores are all NaN has m = -inf and l = NaN)
+        const float f = ml.x != -INFINITY ? fast_exp2(ml.x - M) : 0.0f;
+        L += f * ml.y;
+        if (ml.x != -INFINITY || ml.y != 0.0f)
+          acc += f * *reinterpret_cast<const float4_t *>(&seq_o[w][r * (D + 4) + d]);
+      }
+      const float inv = M == -INFINITY || !(L > 0.0f) ? L * 0.0f : 1.0f / L;
+      const float run[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+      store_run<4>(a.out, out_row_base(a, b0, hk, rbase + r, D) + d, run, a.out_dtype);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -796,20 +835,20 @@ __global__ __launch_bounds__(64 * q4_slices<D>(), 2) void k_attn_q4(AttnArgs a) 
 // ---------------------------------------------------------------------------
 namespace {
 
-template <int D, int NRT>
+template <int D, int NRT, bool SEQ>
 hipError_t launch_q4(const AttnArgs &args, dim3 grid, hipStream_t st) {
   const bool low = args.out_dtype != DT_BF16;
-  const dim3 block(64 * q4_slices<D>());
+  const dim3 block(64 * (SEQ ? kSeqWaves : q4_slices<D>()));
   if (args.window > 0) {
     if (low)
-      k_attn_q4<D, NRT, true, true><<<grid, block, 0, st>>>(args);
+      k_attn_q4<D, NRT, true, true, SEQ><<<grid, block, 0, st>>>(args);
     else
-      k_attn_q4<D, NRT, true, false><<<grid, block, 0, st>>>(args);
+      k_attn_q4<D, NRT, true, false, SEQ><<<grid, block, 0, st>>>(args);
   } else {
     if (low)
-      k_attn_q4<D, NRT, false, true><<<grid, block, 0, st>>>(args);
+      k_attn_q4<D, NRT, false, true, SEQ><<<grid, block, 0, st>>>(args);
     else
-      k_attn_q4<D, NRT, false, false><<<grid, block, 0, st>>>(args);
+      k_attn_q4<D, NRT, false, false, SEQ><<<grid, block, 0, st>>>(args);
   }
   return hipGetLastError();
 }
@@ -818,7 +857,7 @@ template <int D, int NRT>
 int32_t q4_occupancy() {
   static const int32_t n = [] {
     int blocks = 0;
-    const auto *fn = reinterpret_cast<const void *>(&k_attn_q4<D, NRT, false, true>);
+    const auto *fn = reinterpret_cast<const void *>(&k_attn_q4<D, NRT, false, true, false>);
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, fn, 64 * q4_slices<D>(), 0) != hipSuccess || blocks < 1) {
       (void)hipGetLastError();
       blocks = 8 / q4_slices<D>();
@@ -844,21 +883,31 @@ int32_t q4_groups_per_cu(const PoolGeometry &g, int32_t nrt) {
   }
 }
 
+bool q4_per_sequence(const PoolGeometry &g, const AttnLaunch &a, const AttnPlan &p) {
+  if (!p.q4 || g.D > 128 || p.NR > kSeqRows || p.split_blocks > 0 || a.partial_only || a.len_const >= 0 || !a.causal)
+    return false;
+  return (int64_t)a.B * g.Hkv <= g.num_cus && p.nb_cap <= 3 * kSeqWaves;
+}
+
 hipError_t launch_attn_q4(const PoolGeometry &g, int32_t layer, const AttnLaunch &a, const AttnPlan &p, hipStream_t st) {
   if (p.waves < 1 || p.group_waves != 1 || p.rows_per_group != 16 * p.nrt ||
       (int64_t)p.row_groups * p.rows_per_group < p.NR || (a.k_new && a.Lq != 1) || g.Hkv > 65535 || p.row_groups > 65535)
     return hipErrorInvalidValue;
   const AttnArgs args = make_attn_args(g, layer, a, p);
+  if (q4_per_sequence(g, a, p)) {
+    const dim3 seq((unsigned)a.B, (unsigned)g.Hkv);
+    return g.D == 64 ? launch_q4<64, 1, true>(args, seq, st) : launch_q4<128, 1, true>(args, seq, st);
+  }
   const dim3 grid((unsigned)p.waves, (unsigned)g.Hkv, (unsigned)p.row_groups);
   switch (4 * g.D + p.nrt) {
-    case 4 * 64 + 1: return launch_q4<64, 1>(args, grid, st);
-    case 4 * 64 + 2: return launch_q4<64, 2>(args, grid, st);
-    case 4 * 128 + 1: return launch_q4<128, 1>(args, grid, st);
-    case 4 * 128 + 2: return launch_q4<128, 2>(args, grid, st);
-    case 4 * 256 + 1: return launch_q4<256, 1>(args, grid, st);
-    case 4 * 256 + 2: return launch_q4<256, 2>(args, grid, st);
-    case 4 * 512 + 1: return launch_q4<512, 1>(args, grid, st);
-    case 4 * 512 + 2: return launch_q4<512, 2>(args, grid, st);
+    case 4 * 64 + 1: return launch_q4<64, 1, false>(args, grid, st);
+    case 4 * 64 + 2: return launch_q4<64, 2, false>(args, grid, st);
+    case 4 * 128 + 1: return launch_q4<128, 1, false>(args, grid, st);
+    case 4 * 128 + 2: return launch_q4<128, 2, false>(args, grid, st);
+    case 4 * 256 + 1: return launch_q4<256, 1, false>(args, grid, st);
+    case 4 * 256 + 2: return launch_q4<256, 2, false>(args, grid, st);
+    case 4 * 512 + 1: return launch_q4<512, 1, false>(args, grid, st);
+    case 4 * 512 + 2: return launch_q4<512, 2, false>(args, grid, st);
     default: return hipErrorInvalidValue;
   }
 }

@@ -89,6 +89,32 @@ __device__ __forceinline__ uint32_t q4_value_bits(uint32_t c, float s, float b) 
   return f32_to_f16_bits(x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x);
 }
 
+// One slice of a row of K or V (lane: E = D/64 consecutive dims, fp32) as codes:
+// the wave's form.
+template <int D, int DT>
+__device__ __forceinline__ uint32_t q4_quantize_row(const float (&x)[D / 64], uint32_t (&code)[D / 64]) {
+  constexpr int E = D / 64, LPG = 64 / E;
+  float w[E], lo = INFINITY, hi = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    nan |= x[e] != x[e];
+    w[e] = q4_limit<DT>(x[e]);
+    lo = fminf(lo, w[e]);
+    hi = fmaxf(hi, w[e]);
+  }
+  lo = wave_min_range<1, LPG / 2>(lo);
+  hi = wave_max_range<1, LPG / 2>(hi);
+  const uint64_t in_group = (LPG == 64 ? ~0ull : ((1ull << (LPG & 63)) - 1)) << ((threadIdx.x & 63) / LPG * LPG);
+  const bool any = (__ballot(nan) & in_group) != 0;
+  float s, b;
+  const uint32_t meta = q4_params(lo, hi, any, s, b);
+  const float r = __builtin_amdgcn_rcpf(s);
+#pragma unroll
+  for (int e = 0; e < E; ++e) code[e] = q4_code(w[e], s, b, r);
+  return meta;
+}
+
 // ----------------------------------------------------------- matrix operands
 // Codes become fp16 numbers of their own exponent (a subnormal 2^-24 c would be
 // exact as well, but the matrix instructions align their sums to the operands'

@@ -1480,6 +1480,7 @@ hipError_t launch_attention(const PoolGeometry &g, int32_t layer, const AttnLaun
   if (e != hipSuccess) return e;
   // windowed decode kernel at head_dim <= 256: merged inside its workgroups
   if (!p.use_mfma && !p.q4 && a.window > 0 && g.D <= 256) return hipSuccess;
+  if (q4_per_sequence(g, a, p)) return hipSuccess;
   return launch_attn_merge(g, layer, a, p, st);
 }
 

@@ -239,6 +239,65 @@ __global__ __launch_bounds__(256) void k_q4_append(LayerView lv, const uint16_t 
   }
 }
 
+// The same for a few rows (a decode step's tokens, drafts): a wave per row of K or
+// of V, no image and no barrier.
+template <int D, int DT, bool ROPE>
+__global__ __launch_bounds__(256) void k_q4_append_rows(LayerView lv, const uint16_t *__restrict__ k,
+                                                        const uint16_t *__restrict__ v, int64_t sb, int64_t sh,
+                                                        int64_t sl, const int32_t *__restrict__ slots, int32_t B,
+                                                        int32_t L, int32_t H, Q4Rope rope) {
+  constexpr int G = D / 64, E = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (wave >= 2 * (int64_t)B * H * L) return;
+  const int kv = (int)(wave & 1);
+  const int64_t row = wave >> 1;  // [B][L][H]: neighbours share their slot
+  const int h = (int)(row % H), l = (int)(row / H % L), b = (int)(row / H / L);
+  const int64_t at = (int64_t)b * L + l;
+  const int slot = slots[at];
+  const int p = ROPE ? rope.pos[at] : 0;
+  const uint16_t *src = (kv ? v : k) + (int64_t)b * sb + (int64_t)h * sh + (int64_t)l * sl;
+  const int d0 = lane * E;
+  float x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = elem_to_f32<DT>(src[d0 + e]);
+  if (slot < 0 || (slot >> 6) >= lv.num_blocks) return;
+  if constexpr (ROPE) {
+    if ((unsigned)p >= (unsigned)rope.max_pos) return;
+    if (kv == 0) {
+      const float *cs = rope.cs + (int64_t)p * D + (d0 & (D / 2 - 1));
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float y = __shfl_xor(x[e], 32, 64), c = cs[e], sn = cs[D / 2 + e];
+        x[e] = round_dt<DT>(lane >= 32 ? y * sn + x[e] * c : x[e] * c - y * sn);
+      }
+    }
+  }
+  uint32_t code[E];
+  const uint32_t meta = q4_quantize_row<D, DT>(x, code);
+  const int t = slot & 63;
+  uint8_t *reg = head_region(lv, slot >> 6, h);
+  if (kv == 0) {
+    // 8/E lanes hold a word
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) w |= code[e] << (4 * q4_nibble((d0 + e) & 7));
+    if constexpr (E < 8) w |= (uint32_t)__shfl_xor((int)w, 1, 64);
+    if constexpr (E < 4) w |= (uint32_t)__shfl_xor((int)w, 2, 64);
+    if constexpr (E < 2) w |= (uint32_t)__shfl_xor((int)w, 4, 64);
+    if ((d0 & 7) == 0) *reinterpret_cast<uint32_t *>(reg + q4_k_word(D, t, d0 / 8)) = w;
+  } else {
+    // dims d and d + 16 share a byte
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t up = (uint32_t)__shfl_xor((int)code[e], 16 / E, 64);
+      if ((d0 & 16) == 0) reg[q4_v_byte(D, t, 16 * (d0 >> 5) + ((d0 + e) & 15))] = (uint8_t)(code[e] | (up << 4));
+    }
+  }
+  if ((d0 & 63) == 0)
+    *reinterpret_cast<uint32_t *>(reg + (kv ? q4_vm_offset(D) : q4_km_offset(D)) + (t * G + d0 / 64) * 4) = meta;
+}
+
 // ---------------------------------------------------------------------------
 // Read-back as fp16.  A workgroup stages up to 64 rows of one (sequence, KV
 // head) in LDS -- the whole head region where they are one block's -- and
@@ -377,6 +436,24 @@ hipError_t launch_q4_append(const PoolGeometry &g, int32_t layer, const void *k,
   const dim3 grid((unsigned)(((int64_t)L + 126) / 64), (unsigned)g.Hkv, (unsigned)B), block(256);
   const LayerView lv = view_of(g, layer);
   const Q4Rope rope{rope_pos, rope_cs, rope_max_pos};
+  if (L <= 16) {
+    const int64_t waves = 2 * (int64_t)B * g.Hkv * L;
+    const dim3 rows((unsigned)((waves + 3) / 4));
+    KRILL_Q4_DISPATCH(g.D, {
+      if (g.in_dtype == DT_BF16) {
+        if (rope_pos)
+          k_q4_append_rows<D, DT_BF16, true><<<rows, block, 0, st>>>(lv, kk, vv, sb, sh, sl, slots, B, L, g.Hkv, rope);
+        else
+          k_q4_append_rows<D, DT_BF16, false><<<rows, block, 0, st>>>(lv, kk, vv, sb, sh, sl, slots, B, L, g.Hkv, rope);
+      } else {
+        if (rope_pos)
+          k_q4_append_rows<D, DT_F16, true><<<rows, block, 0, st>>>(lv, kk, vv, sb, sh, sl, slots, B, L, g.Hkv, rope);
+        else
+          k_q4_append_rows<D, DT_F16, false><<<rows, block, 0, st>>>(lv, kk, vv, sb, sh, sl, slots, B, L, g.Hkv, rope);
+      }
+    });
+    return hipGetLastError();
+  }
   KRILL_Q4_DISPATCH(g.D, {
     if (g.in_dtype == DT_BF16) {
       if (rope_pos)

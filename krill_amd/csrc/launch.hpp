@@ -133,6 +133,8 @@ int32_t prefill_groups_per_cu(const PoolGeometry &g);
 
 // 16-row tiles per wave and resident workgroups per compute unit of the 4-bit pools' kernel.
 int32_t q4_row_tiles(int32_t NR);
+// Whether a call runs in workgroups per sequence that leave no partial results.
+bool q4_per_sequence(const PoolGeometry &g, const AttnLaunch &a, const AttnPlan &p);
 int32_t q4_groups_per_cu(const PoolGeometry &g, int32_t nrt);
 
 // Per-wave timestamps of the last decode launch (diagnostic build only).

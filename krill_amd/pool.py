@@ -14,10 +14,17 @@ from . import _lib as L
 QUANT_MODES = {"ref_row": L.QUANT_REF_ROW, "affine_g64": L.QUANT_AFFINE_G64, "affine4_g64": L.QUANT_AFFINE4_G64}
 
 
-def _torch():
-    import torch
+_TORCH = None
 
-    return torch
+
+def _torch():
+    """torch, imported on first use (host-only pools run without it)."""
+    global _TORCH
+    if _TORCH is None:
+        import torch
+
+        _TORCH = torch
+    return _TORCH
 
 
 def _dtype_code(dt) -> int:
@@ -71,6 +78,8 @@ class KVPool:
         self.quant_mode = quant_mode
         self.mode = QUANT_MODES[quant_mode]
         self.in_dtype_code = _dtype_code(in_dtype)
+        self._in_dtype = _torch_dtype(self.in_dtype_code)
+        self._needs = {}
         self.groups = 1 if self.mode == L.QUANT_REF_ROW else head_dim // 64
         self.code_bits = 4 if self.mode == L.QUANT_AFFINE4_G64 else 8
         self.host_only = host_only
@@ -79,6 +88,8 @@ class KVPool:
                           float(evict_watermark), int(max_prefix_entries), int(min_prefix_len),
                           int(max_entry_bytes), int(free_list_seed))
         self._h = ctypes.c_void_p()
+        # the device krill_pool_create puts the pool on: the current one
+        self._device = _torch().cuda.current_device() if not host_only and _torch().cuda.is_available() else None
         st = ctypes.c_void_p(stream) if stream else None
         L.check(L.lib().krill_pool_create(ctypes.byref(desc), st, ctypes.byref(self._h)))
 
@@ -116,6 +127,7 @@ class KVPool:
         return out
 
     def set_option(self, option: int, value: int):
+        self._needs.clear()
         L.check(L.lib().krill_pool_set_option(self._h, option, int(value)))
 
     def flush(self, stream=None):
@@ -220,30 +232,43 @@ class KVPool:
         return out.value
 
     # ---------------------------------------------------------- kernels
-    @staticmethod
-    def _stream(stream=None):
-        """hipStream_t for a torch stream, a raw handle (int) or None (torch's current stream)."""
+    def _stream(self, stream=None):
+        """hipStream_t for a torch stream, a raw handle (int) or None (torch's current stream on the
+        pool's device; read from torch's C layer: torch.cuda.current_stream() builds a stream object,
+        8 us of the host's time per call)."""
         if stream is not None:
-            return ctypes.c_void_p(getattr(stream, "cuda_stream", stream))
-        torch = _torch()
-        if torch.cuda.is_available():
-            return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-        return None
+            return getattr(stream, "cuda_stream", stream)
+        if self._device is None:
+            return None
+        return _torch()._C._cuda_getCurrentRawStream(self._device)
 
     def _check_dev(self, name, t, dtype=None, shape=None):
-        torch = _torch()
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        if not isinstance(t, _torch().Tensor) or not t.is_cuda:
             raise ValueError(f"{name} must be a CUDA (HIP) tensor")
+        if t.get_device() != self._device:
+            raise ValueError(f"{name} is on device {t.get_device()}, the pool on device {self._device}")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
         if dtype is not None and t.dtype != dtype:
             raise ValueError(f"{name} has dtype {t.dtype}, expected {dtype}")
-        if shape is not None and tuple(t.shape) != tuple(shape):
+        if shape is not None and t.shape != tuple(shape):
             raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
     @property
     def in_dtype(self):
-        return _torch_dtype(self.in_dtype_code)
+        return self._in_dtype
+
+    def _need(self, fn, *args) -> int:
+        """Workspace bytes of a call (they depend on the pool, its options and the arguments)."""
+        key = (fn, *args)
+        n = self._needs.get(key)
+        if n is None:
+            out = ctypes.c_size_t()
+            L.check(getattr(L.lib(), fn)(self._h, *args, ctypes.byref(out)))
+            if len(self._needs) > 4096:
+                self._needs.clear()
+            n = self._needs[key] = out.value
+        return n
 
     def quantize_append(self, layer: int, k, v, slot_mapping, stream=None):
         """k, v: [B, Hkv, L, D] in in_dtype; slot_mapping: int32 [B, L] (device)."""
@@ -360,15 +385,10 @@ class KVPool:
         L.check(L.lib().krill_copy_blocks(self._h, src_dst.data_ptr(), src_dst.numel() // 2, self._stream(stream)))
 
     def workspace_size(self, B: int, Hq: int, Lq: int, max_seq_len: int) -> int:
-        out = ctypes.c_size_t()
-        L.check(L.lib().krill_attention_workspace_size(self._h, B, Hq, Lq, max_seq_len, ctypes.byref(out)))
-        return out.value
+        return self._need("krill_attention_workspace_size", B, Hq, Lq, max_seq_len)
 
     def shared_prefix_workspace_size(self, B: int, Hq: int, prefix_blocks: int, max_suffix_len: int) -> int:
-        out = ctypes.c_size_t()
-        L.check(L.lib().krill_shared_prefix_workspace_size(self._h, B, Hq, prefix_blocks, max_suffix_len,
-                                                           ctypes.byref(out)))
-        return out.value
+        return self._need("krill_shared_prefix_workspace_size", B, Hq, prefix_blocks, max_suffix_len)
 
     def attention(self, layer: int, q, tables, lens, max_seq_len: int, scale: float, out_dtype=None,
                   ws=None, out=None, stream=None):
@@ -418,10 +438,9 @@ class KVPool:
             out = torch.empty((B, Hq, Lq, D), dtype=out_dtype, device=q.device)
         else:
             self._check_dev("out", out, out_dtype, (B, Hq, Lq, D))
-        need = ctypes.c_size_t()
-        L.check(L.lib().krill_window_workspace_size(self._h, B, Hq, Lq, mb, max_seq_len, window, ctypes.byref(need)))
-        if ws is None or ws.numel() < need.value:
-            ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device=q.device)
+        need = self._need("krill_window_workspace_size", B, Hq, Lq, mb, max_seq_len, window)
+        if ws is None or ws.numel() < need:
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
         L.check(L.lib().krill_attention_windowed(
             self._h, layer, q.data_ptr(), Lq, tables.data_ptr(), lens.data_ptr(),
             starts.data_ptr() if starts is not None else None, window, B, mb, max_seq_len, Hq, float(scale),
@@ -462,10 +481,9 @@ class KVPool:
             out = torch.empty((B, Hq, 1, D), dtype=out_dtype, device=q.device)
         else:
             self._check_dev("out", out, out_dtype, (B, Hq, 1, D))
-        need = ctypes.c_size_t()
-        L.check(L.lib().krill_window_workspace_size(self._h, B, Hq, 1, mb, max_seq_len, window, ctypes.byref(need)))
-        if ws is None or ws.numel() < need.value:
-            ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device=q.device)
+        need = self._need("krill_window_workspace_size", B, Hq, 1, mb, max_seq_len, window)
+        if ws is None or ws.numel() < need:
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
         L.check(L.lib().krill_decode_append_attention_windowed(
             self._h, layer, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), H * D, D, tables.data_ptr(),
             lens.data_ptr(), starts.data_ptr() if starts is not None else None, window, B, mb, max_seq_len, Hq,
@@ -498,10 +516,9 @@ class KVPool:
             out = torch.empty((B, Hq, 1, D), dtype=out_dtype, device=q.device)
         else:
             self._check_dev("out", out, out_dtype, (B, Hq, 1, D))
-        need = ctypes.c_size_t()
-        L.check(L.lib().krill_shared_prefix_workspace_size(self._h, B, Hq, P, max_suffix_len, ctypes.byref(need)))
-        if ws is None or ws.numel() < need.value:
-            ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device=q.device)
+        need = self._need("krill_shared_prefix_workspace_size", B, Hq, P, max_suffix_len)
+        if ws is None or ws.numel() < need:
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
         if k_new is None:
             L.check(L.lib().krill_decode_attention_shared_prefix(
                 self._h, layer, q.data_ptr(), prefix_table.data_ptr(), P, suffix_tables.data_ptr(),
