@@ -38,15 +38,24 @@
 
 namespace krill {
 
+// Of a 4-bit pool this kernel has two forms.  MODE_AFFINE4 keeps the codes exact
+// (c - 8) and the scales in fp32, as MODE_AFFINE does.  MODE_DEQ4, for bf16
+// outputs, holds K and V dequantized and rounded to fp16 (values halved, so that a
+// group of the whole fp16 range does not overflow) and weights as one fp16 number:
+// 2^-11 of a value each against the output's half step of 2^-8.  Scales then cost
+// nothing per (row, key) and P.V half the products.
+enum { MODE_DEQ4 = 3 };
+
 // One workgroup's LDS: fp16 K tile [token][d], fp16 V^T tile [d][position],
 // rows padded by 16 bytes (the 8 rows a group of lanes reads start in
 // different banks), and the blocks' scales.
 template <int D, int MODE>
 struct PrefillLds {
-  static constexpr int G = MODE != MODE_REF ? D / 64 : 1;
+  static constexpr bool DEQ = MODE == MODE_DEQ4;
+  static constexpr int G = MODE != MODE_REF && !DEQ ? D / 64 : 1;
   static constexpr int KTS = D * 2 + 16, VTS = 64 * 2 + 16;
   static constexpr int GZ = (G + 3) / 4 * 4;  // groups of the zero-point contraction
-  static constexpr bool AFF = MODE != MODE_REF;
+  static constexpr bool AFF = MODE != MODE_REF && !DEQ;
   __attribute__((aligned(16))) uint8_t k[64 * KTS];
   __attribute__((aligned(16))) uint8_t v[D * VTS];
   __attribute__((aligned(16))) float ks[AFF ? G * 64 : 4];      // [g][token]: s times the softmax scale
@@ -54,6 +63,7 @@ struct PrefillLds {
   __attribute__((aligned(16))) float vz[AFF ? G * 64 : 4];      // [g][position]: z + 128 s
   __attribute__((aligned(16))) _Float16 vs[AFF ? G * 64 : 8];   // [g][position]
   int big;  // last block with a V scale past kBigScale
+  __attribute__((aligned(16))) _Float16 ds[2][DEQ ? D : 8], dz[2][DEQ ? D : 8];  // DEQ: V's s / 2 and (b + 8 s) / 2, [g][position]
 };
 
 __device__ __forceinline__ float4_t mfma16x16x4f32(float a, float b, float4_t c) {
@@ -138,7 +148,8 @@ constexpr int prefill_min_waves() { return NRT * D >= 512 ? 1 : 2; }
 // VAR: 0 plain; 1 RoPE of the queries; 2 sliding window.
 template <int D, int MODE, int NRT, int VAR>
 __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_prefill(AttnArgs a) {
-  constexpr bool ROPE = VAR == 1, WIN = VAR == 2, AFF = MODE != MODE_REF, Q4 = MODE == MODE_AFFINE4;
+  constexpr bool ROPE = VAR == 1, WIN = VAR == 2, DEQ = MODE == MODE_DEQ4, AFF = MODE != MODE_REF && !DEQ,
+                 Q4 = MODE == MODE_AFFINE4 || DEQ;
   constexpr int G = AFF ? D / 64 : 1;
   constexpr int GZ4 = (G + 3) / 4;
   constexpr int KS = D / 32;      // 32-d steps of Q.K^T
@@ -149,6 +160,9 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
   // wid + W k of the region's D / 16, K's before V's)
   constexpr int KP = D / 16 / W;
   constexpr int VP = Q4 ? 0 : D / 16 / W;
+  constexpr int GD = D / 64;      // scale groups of the pool's layout (4 bits)
+  constexpr int KQ = D / 64 >= 2 ? KP / 2 : KP;  // 4 bits: a thread's pieces that can be K's
+  constexpr int VM = (GD + 3) / 4;               // DEQ: words of V's metadata per thread
   constexpr int MW = AFF ? (128 * G + 64 * W - 1) / (64 * W) : 0;  // metadata words per thread
   static_assert(W == 4 && D % 64 == 0, "a wave per (token group, half) of V");
   static_assert(Q4 || prefill_loads_inside<D, G>(KP, VP, MW), "a block's loads stay in its head region");
@@ -232,6 +246,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
   uint4 kraw[KP], vraw[VP > 0 ? VP : 1];
   uint32_t mraw[AFF ? MW : 1];  // affine: words tid + 64 W k of the block's metadata; row mode: K word of token `lane`
   uint32_t vmeta = 0u;          // row mode: V word of token `lane`
+  uint32_t kword[DEQ ? KQ : 1][2], vword[DEQ ? VM : 1];  // DEQ: K's words of a piece's halves, V's words tid + 256 k
   const int vlane = prefill_v_lane<D>(lane);
   auto issue = [&](int i) {
     // after the last block: an empty resource (the offsets in scalars may escape
@@ -253,9 +268,36 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
       for (int k = 0; k < MW; ++k)
         mraw[k] = __builtin_amdgcn_raw_buffer_load_b32(
             r, lane * 4, prefill_meta_piece<D, G>(wid, k) - (Q4 ? km_offset(D) - q4_km_offset(D) : 0), 0);
+    } else if constexpr (DEQ) {
+#pragma unroll
+      for (int k = 0; k < VM; ++k)
+        vword[k] = __builtin_amdgcn_raw_buffer_load_b32(r, q4_vm_offset(D) + 4 * ((tid + 256 * k) & (64 * GD - 1)), 0, 0);
+#pragma unroll
+      for (int k = 0; k < KQ; ++k) {
+        const int piece = (wid + W * k) & (D / 32 - 1);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int t = D == 64 ? 32 * piece + 16 * hf + n : 16 * (piece / (D / 128 > 0 ? D / 128 : 1)) + n;
+          const int g = D == 64 ? 0 : 2 * (piece % (D / 128 > 0 ? D / 128 : 1)) + hf;
+          kword[k][hf] = __builtin_amdgcn_raw_buffer_load_b32(r, q4_km_offset(D) + 4 * (t * GD + g), 0, 0);
+        }
+      }
     } else {
       mraw[0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, km_offset(D), 0);
       vmeta = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, vm_offset(D, G), 0);
+    }
+  };
+
+  // DEQ: V's scales of block i, before it is converted (the words have arrived)
+  auto stage_v = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < (DEQ ? VM : 0); ++k) {
+      const int m = tid + 256 * k, t = m / GD, g = m % GD, p = (t & 32) + vpos(t & 31);
+      const float s = f16_bits_to_f32((uint16_t)(vword[k] & 0xffffu)), z = f16_bits_to_f32((uint16_t)(vword[k] >> 16));
+      if (m < 64 * GD) {
+        lds.ds[i & 1][64 * g + p] = (_Float16)(0.5f * s);
+        lds.dz[i & 1][64 * g + p] = (_Float16)(0.5f * __builtin_fmaf(8.0f, s, z));
+      }
     }
   };
 
@@ -267,13 +309,13 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
   float q_up[AFF ? 1 : NRT];
   float q_dn[AFF ? NRT : 1];  // affine: 2^-k alone
   bool any_up = false;        // affine: some row of the wave has a 2^k other than 1
-  float q_bad[AFF ? NRT : 1]; // affine: NaN where the row holds an infinity or NaN, else 0
+  float q_bad[AFF || DEQ ? NRT : 1]; // affine, 4 bits: NaN where the row holds an infinity or NaN, else 0
   bool rvalid[NRT];
 #pragma unroll
   for (int rt = 0; rt < NRT; ++rt) rvalid[rt] = rbase + 16 * rt + n < a.NR;
   // row mode: the sign of the scale goes to the queries (zero scale: zero queries)
   const float qsign = AFF || a.scale_log2 > 0.0f ? 1.0f : a.scale_log2 < 0.0f ? -1.0f : 0.0f;
-  const float qscale = AFF || qsign == 0.0f ? 1.0f : fabsf(a.scale_log2);
+  const float qscale = AFF || qsign == 0.0f ? 1.0f : fabsf(a.scale_log2) * (DEQ ? 2.0f : 1.0f);
   auto load_q = [&](int bq) {
     bool ups = false;
 #pragma unroll
@@ -324,7 +366,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
         mx = fmaxf(mx, shfl_xor(mx, 32));
         down = q_range_scale(mx, up);
       }
-      q_up[rt] = qscale * up;
+      if constexpr (!AFF) q_up[rt] = qscale * (DEQ ? fminf(up, 0x1p80f) : up);  // (DEQ: see below)
       // (4 bits: rows past about 2^95 take their scores some powers of two too small,
       // so that nothing overflows; scores that differ do so by far more than the
       // softmax resolves either way)
@@ -355,6 +397,12 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
           qsum[AFF ? ks / 2 : 0] += (float)hl + (float)hh;
         }
         qB[rt][ks] = v;
+      }
+      if constexpr (DEQ) {
+        float bad = qsum[0] * 0.0f;
+        bad += shfl_xor(bad, 16);
+        bad += shfl_xor(bad, 32);
+        q_bad[rt] = bad;
       }
       if constexpr (AFF) {
 #pragma unroll
@@ -411,6 +459,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
   if (AFF && tid == 0) lds.big = -1;
   issue(i0);
   load_q(b);
+  if constexpr (DEQ) stage_v(i0);
 
   float one = 1.0f;
   asm volatile("" : "+v"(one));
@@ -469,7 +518,25 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
         for (int k = 0; k < KP; ++k) {
           const int piece = wid + W * k;
           const uint32_t w4[4] = {kraw[k].x, kraw[k].y, kraw[k].z, kraw[k].w};
-          if (piece < D / 32) {
+          if (DEQ && piece < D / 32) {
+            half2_t s2[2], z2[2];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              const uint32_t m = kword[DEQ && k < KQ ? k : 0][hf];
+              const float s = f16_bits_to_f32((uint16_t)(m & 0xffffu)), zb = f16_bits_to_f32((uint16_t)(m >> 16));
+              const _Float16 sh = (_Float16)(0.5f * s), zh = (_Float16)(0.5f * __builtin_fmaf(8.0f, s, zb));
+              s2[hf] = half2_t{sh, sh};
+              z2[hf] = half2_t{zh, zh};
+            }
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int tg = D == 64 ? 2 * piece + (w >> 1) : piece / (D / 128 > 0 ? D / 128 : 1);
+              const int g = D == 64 ? 0 : 2 * (piece % (D / 128 > 0 ? D / 128 : 1)) + (w >> 1);
+              *reinterpret_cast<half8_t *>(lds.k + (16 * tg + nn) * KTS + (64 * g + 16 * qq + 8 * (w & 1)) * 2) =
+                  q4_scaled(q4_k_operand(w4[w], magic), q4_join(s2[w >> 1], s2[w >> 1], s2[w >> 1], s2[w >> 1]),
+                            q4_join(z2[w >> 1], z2[w >> 1], z2[w >> 1], z2[w >> 1]));
+            }
+          } else if (piece < D / 32) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               const int tg = D == 64 ? 2 * piece + (w >> 1) : piece / (D / 128);
@@ -483,6 +550,24 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
             for (int ks = 0; ks < 2; ++ks) {
               half8_t lo, hi;
               q4_v_operands(w4[2 * ks], w4[2 * ks + 1], magic, lo, hi);
+              if constexpr (DEQ) {
+                // (dims 32 j + n and 32 j + 16 + n: group j / 2)
+                const int at = 64 * ((piece - D / 32) >> 1) + 32 * ks + 8 * qq;
+                half8_t s8 = *reinterpret_cast<const half8_t *>(&lds.ds[i & 1][at]);
+                half8_t z8 = *reinterpret_cast<const half8_t *>(&lds.dz[i & 1][at]);
+                if (tbase + 64 > len || (WIN && tbase < wst)) {
+                  // rows past the sequence's end or below the window are not data
+#pragma unroll
+                  for (int x = 0; x < 8; ++x) {
+                    const int t = tbase + 32 * ks + 4 * qq + (x & 3) + 16 * (x >> 2);
+                    const bool data = t < len && (!WIN || t >= wst);
+                    s8[x] = data ? s8[x] : (_Float16)0.0f;
+                    z8[x] = data ? z8[x] : (_Float16)0.0f;
+                  }
+                }
+                lo = q4_scaled(lo, s8, z8);
+                hi = q4_scaled(hi, s8, z8);
+              }
               *reinterpret_cast<half8_t *>(o + 64 * ks) = lo;
               *reinterpret_cast<half8_t *>(o + 16 * VTS + 64 * ks) = hi;
             }
@@ -523,7 +608,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
             if (data && fabsf(sf) > kBigScale) lds.big = i;
           }
         }
-      } else {
+      } else if constexpr (!DEQ) {
         const half2_t m1024 = half2_t{(_Float16)-1024.0f, (_Float16)-1024.0f};
         const _Float16 sk = __builtin_bit_cast(_Float16, (uint16_t)(mraw[0] & 0xffffu));
         const _Float16 zk = __builtin_bit_cast(_Float16, (uint16_t)(mraw[0] >> 16));
@@ -768,8 +853,10 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
         }
       };
       ldvm(mv, 0, 0);
+      if constexpr (DEQ) stage_v(i + 1);  // (visible at the next block's first barrier)
+      constexpr int NM = DEQ ? 4 : 8;  // products a tile: DEQ has no low parts
 #pragma unroll
-      for (int part = 0; part < 8 * NRT; ++part) build(0, part);
+      for (int part = 0; part < 8 * NRT; part += DEQ ? 2 : 1) build(0, part);
       if constexpr (AFF) ldvm(mv, 1 / NSL, 1 % NSL);
 #pragma unroll
       for (int u = 0; u < 2 * NSL; ++u) {
@@ -779,14 +866,14 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
         if (u + 1 < 2 * NSL) ldv(fr[(F0 + u + 1) & 1], (u + 1) / NSL, (u + 1) % NSL);
         fence_lds();
 #pragma unroll
-        for (int m = 0; m < 8 * NRT; ++m) {
+        for (int m = 0; m < NM * NRT; ++m) {
           const int j = m / NRT % 4, rt = m % NRT;
           oacc[rt][4 * sl + j] =
               mfma16x16x32(fr[(F0 + u) & 1][j], m < 4 * NRT ? Bh[bb][rt] : Bl[bb][rt], oacc[rt][4 * sl + j]);
           if (next && m > 0) {
             fence_all();
-            build(u + 1, m - 1);
-            if (m == 8 * NRT - 1) build(u + 1, m);
+            build(u + 1, DEQ ? 2 * (m - 1) : m - 1);
+            if (m == NM * NRT - 1) build(u + 1, DEQ ? 2 * m : m);
             fence_all();
           }
         }
@@ -812,10 +899,10 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
         float c = c_part[rt][g];
         c += shfl_xor(c, 16);
         c += shfl_xor(c, 32);
-        cg[g] = AFF ? c + q_bad[AFF ? rt : 0] : c;  // (a NaN score would be lost in the running reference)
+        cg[g] = AFF || DEQ ? c + q_bad[AFF || DEQ ? rt : 0] : c;  // (a NaN score would be lost in the running reference)
       }
       if (!rvalid[rt]) continue;
-      const float mul = !whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+      const float mul = (DEQ ? 2.0f : 1.0f) * (!whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f);
       const int64_t pi = slot * RR + 16 * rt + n;
       const int64_t ob = (whole ? out_row_base(a, b, hk, rbase + 16 * rt + n, D) : pi * D) + 4 * q4;
       auto put = [&](void *out, auto dtype) {
@@ -887,11 +974,12 @@ hipError_t launch_attn_prefill(const PoolGeometry &g, int32_t layer, const AttnL
   if ((int64_t)p.waves * g.Hkv * groups > INT32_MAX) return hipErrorInvalidValue;
   const AttnArgs args = make_attn_args(g, layer, a, p);
   if (g.mode == MODE_AFFINE4) {
+    const bool deq = args.out_dtype == DT_BF16;
     switch (g.D) {
-      case 64: return launch_prefill_dm<64, MODE_AFFINE4>(args, p, st);
-      case 128: return launch_prefill_dm<128, MODE_AFFINE4>(args, p, st);
-      case 256: return launch_prefill_dm<256, MODE_AFFINE4>(args, p, st);
-      case 512: return launch_prefill_dm<512, MODE_AFFINE4>(args, p, st);
+      case 64: return deq ? launch_prefill_dm<64, MODE_DEQ4>(args, p, st) : launch_prefill_dm<64, MODE_AFFINE4>(args, p, st);
+      case 128: return deq ? launch_prefill_dm<128, MODE_DEQ4>(args, p, st) : launch_prefill_dm<128, MODE_AFFINE4>(args, p, st);
+      case 256: return deq ? launch_prefill_dm<256, MODE_DEQ4>(args, p, st) : launch_prefill_dm<256, MODE_AFFINE4>(args, p, st);
+      case 512: return deq ? launch_prefill_dm<512, MODE_DEQ4>(args, p, st) : launch_prefill_dm<512, MODE_AFFINE4>(args, p, st);
       default: return hipErrorInvalidValue;
     }
   }

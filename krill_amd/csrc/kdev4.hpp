@@ -166,4 +166,10 @@ __device__ __forceinline__ void q4_v_operands(uint32_t w0, uint32_t w1, uint32_t
                                          q4_centred_hi(u1, magic)});
 }
 
+// Eight centred codes as the values they stand for, s (c - 8) + z rounded to fp16.
+__device__ __forceinline__ half8_t q4_scaled(half8_t c, half8_t s, half8_t z) { return __builtin_elementwise_fma(c, s, z); }
+__device__ __forceinline__ half8_t q4_join(half2_t a, half2_t b, half2_t c, half2_t d) {
+  return __builtin_bit_cast(half8_t, uint4{h2_as_u32(a), h2_as_u32(b), h2_as_u32(c), h2_as_u32(d)});
+}
+
 }  // namespace krill

@@ -61,7 +61,7 @@ def weight_error(G):
     return (6 * G + 4) * 2.0 ** -24 * 8 + 2.0 ** -19
 
 
-def bound(q, k, v, scale, want, out, sk=0.0, sv=0.0):
+def bound(q, k, v, scale, want, out, sk=0.0, sv=0.0, long=False):
     """Largest error a row of the kernels' output may show, given float64 q [n, D], k, v [T, D].
 
     Queries and codes enter the products exactly, so a score errs by the roundings of its sums: per
@@ -72,7 +72,9 @@ def bound(q, k, v, scale, want, out, sk=0.0, sv=0.0):
     bf16 outputs: weights are rounded to fp16 (2^-11) and weigh |c - 8| s <= 8 sv, sv the largest
     scale of V; codes of K enter as 1024 + c or 1024 + 16 c (over 16 queries), so a group's three
     sums of products, from the offset's start to two matrix steps, are at most 2^-23 of 1040 times
-    the group's |q| off, in units of the scale, sk the largest."""
+    the group's |q| off, in units of the scale, sk the largest.  Long windows hold k and v as fp16
+    numbers s (c - 8) + z, z = b + 8 s rounded too: 2^-11 of |k| and of |z| <= |k| + 8 sk, and
+    weights of 2^-11."""
     G = k.shape[-1] // 64
     terms = np.abs(q) @ np.abs(k).max(0) * 2.0  # |s c| and |b| are each at most twice the value's range
     dx = (6 * G + 4) * 2.0 ** -23 * terms * abs(scale) * np.log2(np.e)
@@ -80,6 +82,10 @@ def bound(q, k, v, scale, want, out, sk=0.0, sv=0.0):
     if out == "bf16":
         dx = dx + 3 * 2.0 ** -23 * 1040 * np.abs(q).sum(-1) * sk * abs(scale) * np.log2(np.e)
         low = 2.0 ** -11 * 8 * sv
+        if long:
+            kmax, vmax = np.abs(k).max(), np.abs(v).max()
+            dx = dx + 2.0 ** -11 * np.abs(q).sum(-1) * (2 * kmax + 8 * sk) * abs(scale) * np.log2(np.e)
+            low = 2.0 ** -11 * (3 * vmax + 8 * sv)
     vmax = 2.0 * np.abs(v).max()
     rel = 2 * np.log(2.0) * dx + 2.0 ** -19
     return (rel * vmax)[:, None] + low + 0.5 * EPS[out] * np.abs(want) + 2.0 ** -25

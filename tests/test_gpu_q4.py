@@ -48,7 +48,7 @@ class Cache:
         t, n = self.pool.batch_tables(self.seqs, mb)
         return i32(t), i32(n)
 
-    def check(self, got, qbits, scale, out, window=0, upto=None):
+    def check(self, got, qbits, scale, out, window=0, upto=None, long=False):
         """got [B, Hq, Lq, D] against 64 bits, queries at the sequences' last positions."""
         B, Hq, Lq, D = qbits.shape
         H = self.pool.num_kv_heads
@@ -70,7 +70,7 @@ class Cache:
                     assert not g.any()
                     continue
                 err, lim = np.abs(g - want), Q.bound(rows, kd, vd, scale, want, out, *(
-                    Q.quantize(x[b][h], self.dt)[1].max(initial=0) for x in (self.k, self.v)))
+                    Q.quantize(x[b][h], self.dt)[1].max(initial=0) for x in (self.k, self.v)), long=long)
                 assert np.all(err <= lim), f"b {b} h {h}: {np.nanmax(err / lim):.3g} times the bound"
                 # errors of the weights are independent, as the values they weigh: both sum alike
                 x = np.abs(rows @ kd.T).max() * abs(scale) * np.log2(np.e)
@@ -697,4 +697,37 @@ def test_refusals():
         two.attention(0, q, t, n, 64, 1.0)
     assert e.value.code == L.KRILL_E_INVAL
     two.close()
+    pool.close()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("Lq,R,window", [(2, 1, 0), (70, 3, 0), (200, 1, 0), (70, 2, 50), (70, 1, 100)])
+def test_long_windows_with_bf16_outputs(D, Lq, R, window):
+    """The long-window kernel's form for bf16 outputs; slots behind the sequences hold NaN and infinities, one
+    row of the queries a NaN."""
+    from krill_amd import _lib as L
+
+    rng = np.random.default_rng(Lq + window)
+    H, dt, scale = 2, "bf16", 1 / np.sqrt(D)
+    lens = [Lq, Lq + 100, 64 * ((Lq + 63) // 64) + 1, 333]
+    pool = make_pool(H, D, 40, dt)
+    pool.set_option(L.OPT_ATTN_PATH, 2)
+    junk = np.array([0x7fc0, 0x7f80, 0xff80, 0x7f7f], np.uint16)[rng.integers(0, 4, (1, H, pool.num_blocks * 64, D))]
+    pool.quantize_append(0, to_dev(junk, dt), to_dev(junk, dt), all_slots(pool))
+    c = Cache(pool, lens, rng, dt)
+    qb = rand_bits(rng, (len(lens), H * R, Lq, D), dt)
+    t, n = c.tables()
+
+    def run():
+        if window:
+            return pool.attention_windowed(0, to_dev(qb, dt), t, n, None, window, max(lens), scale, out_dtype=torch.bfloat16)
+        return pool.attention(0, to_dev(qb, dt), t, n, max(lens), scale, out_dtype=torch.bfloat16)
+
+    clean = run()
+    c.check(clean, qb, scale, "bf16", window, long=True)
+    qb[1, 0, Lq // 2, 3] = 0x7fc0
+    got = run()
+    assert torch.isnan(got[1, 0, Lq // 2]).all()
+    got[1, 0, Lq // 2] = clean[1, 0, Lq // 2]
+    same(got.float().cpu().numpy(), clean.float().cpu().numpy())
     pool.close()
