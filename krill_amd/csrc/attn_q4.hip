@@ -83,6 +83,8 @@ __device__ __forceinline__ uint32_t rest2(float w0, float w1, uint32_t h, float 
 // lanes' writes before other lanes' reads.
 __device__ __forceinline__ void wave_sync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
 __device__ __forceinline__ void set_word(uint4 &v, int w, uint32_t x) {
   (w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w) = x;
@@ -98,6 +100,10 @@ constexpr float kGap = 5.0f, kOver = 8.0f, kBig = 255.0f;
 
 constexpr int kSeqWaves = 8, kSeqRows = 8;
 
+// Waves per SIMD the registers are budgeted for.
+template <int D, int NRT, bool SEQ>
+constexpr int q4_waves() { return NRT == 1 ? 2 : 1; }
+
 }  // namespace
 
 // NRT: tiles of 16 query rows per wave.  WIN: sliding window.  LOW: the weights'
@@ -105,7 +111,7 @@ constexpr int kSeqWaves = 8, kSeqRows = 8;
 // per (sequence, KV head), each a share of its blocks, their partial results
 // combined in LDS (at most kSeqRows query rows, head_dim up to 128).
 template <int D, int NRT, bool WIN, bool LOW, bool SEQ>
-__global__ __launch_bounds__(64 * (SEQ ? kSeqWaves : q4_slices<D>()), 2) void k_attn_q4(AttnArgs a) {
+__global__ __launch_bounds__(64 * (SEQ ? kSeqWaves : q4_slices<D>()), (q4_waves<D, NRT, SEQ>())) void k_attn_q4(AttnArgs a) {
   static_assert(!SEQ || (NRT == 1 && D <= 128), "one slice, one row tile");
   constexpr int DS = q4_slices<D>(), DW = D / DS;
   constexpr int GD = D / 64;    // groups of a row
@@ -130,6 +136,21 @@ __global__ __launch_bounds__(64 * (SEQ ? kSeqWaves : q4_slices<D>()), 2) void k_
   // (range w of the heads goes to different XCDs)
   const int wv = (int)((blockIdx.x + (unsigned)hk) % gridDim.x);
   const int rbase = rg * RR;
+  // the lane's rows: query position and head of the KV group (divided by way of
+  // floats, put right by at most one: while the lengths are on their way)
+  int rj[NRT], rh[NRT];
+  bool rvalid[NRT];
+  const int j_first = rbase / a.R, j_last = (min(a.NR, rbase + RR) - 1) / a.R;
+#pragma unroll
+  for (int rt = 0; rt < NRT; ++rt) {
+    const int r = rbase + 16 * rt + n;
+    rvalid[rt] = r < a.NR;
+    int j = (int)((float)r * __builtin_amdgcn_rcpf((float)a.R)), h = r - j * a.R;
+    if (h < 0) h += a.R, --j;
+    if (h >= a.R) h -= a.R, ++j;
+    rj[rt] = rvalid[rt] ? j : 0;
+    rh[rt] = rvalid[rt] ? h : 0;
+  }
 
   // ---- flat blocks [i0, iend) of the (head, row group) order
   int c0 = 0, lenv = 0, i0 = 0, iend = 0;
@@ -241,9 +262,6 @@ __global__ __launch_bounds__(64 * (SEQ ? kSeqWaves : q4_slices<D>()), 2) void k_
   float ksf = 1.0f;    // what s and b of K take
   bool any_rd = false;
   float qoff[LOW ? 1 : NRT][G];  // !LOW: what the codes' offsets add to a group's products
-  bool rvalid[NRT];
-#pragma unroll
-  for (int rt = 0; rt < NRT; ++rt) rvalid[rt] = rbase + 16 * rt + n < a.NR;
   // ---- the step's new token, where this range holds the sequence's last block:
   // quantized into LDS, patched into the registers when its block comes up,
   // stored by row group 0 at the segment's end
@@ -358,60 +376,66 @@ __global__ __launch_bounds__(64 * (SEQ ? kSeqWaves : q4_slices<D>()), 2) void k_
   asm volatile("" : "+v"(one));
   const uint32_t magic = q4_magic();
   int i = i0;
-  while (!SEQ || i0 < iend) {
-    // ---- the segment's queries and new token, ahead of the range's first block
-    const bool own = owns_new(b, s);
-    if (own) load_new(b);
-    // (the row's largest |q| over all slices, the queries the slice's turn with)
-    uint4 raw[NRT][2 * G], raw2[NRT][2 * G];
-    float mxr[NRT], mxw = 0.0f;
-    auto elem = [&](uint32_t w, int hf) -> float {
-      const uint16_t u = (uint16_t)(w >> (16 * hf));
-      return a.q_dtype == DT_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
-    };
-    auto largest = [&](const uint4 &v, float m) -> float {
+  // ---- a segment's queries as they come, those that they turn with (another
+  // slice's), its new token: ahead of the range's first block, later ahead of the
+  // segment before's results
+  constexpr int HALF = DW == D ? 0 : DS / 2;  // slices to the dims that turn together
+  uint4 raw[NRT][2 * G], raw2[NRT][2 * G];
+  const uint16_t *qp[NRT];
+  bool own = false;
+  auto q_piece = [&](int rt, int slice, int k) -> uint4 {
+    return *reinterpret_cast<const uint4 *>(qp[rt] + slice * DW + 64 * (k >> 1) + 8 * (k & 1));
+  };
+  auto issue_q = [&](int bs, int ss) {
+    own = owns_new(bs, ss);
+    if (own) load_new(bs);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) m = fmaxf(m, fmaxf(fabsf(elem(word_of(v, w), 0)), fabsf(elem(word_of(v, w), 1))));
-      return m;
-    };
-    auto q_piece = [&](int rt, int slice, int k) -> uint4 {
-      const int r = rvalid[rt] ? rbase + 16 * rt + n : 0;
-      const uint16_t *qp = q_row(a, b, hk * a.R + r % a.R, r / a.R) + slice * DW + 16 * q4;
-      return *reinterpret_cast<const uint4 *>(qp + 64 * (k >> 1) + 8 * (k & 1));
-    };
-    constexpr int HALF = DW == D ? 0 : DS / 2;  // slices to the dims that turn together
-#pragma unroll
-    for (int rt = 0; rt < NRT; ++rt)
+    for (int rt = 0; rt < NRT; ++rt) {
+      qp[rt] = q_row(a, bs, hk * a.R + rh[rt], rj[rt]) + 16 * q4;
 #pragma unroll
       for (int k = 0; k < 2 * G; ++k) {
         raw[rt][k] = q_piece(rt, sl, k);
         raw2[rt][k] = uint4{0u, 0u, 0u, 0u};
         if (HALF && a.rope_cs) raw2[rt][k] = q_piece(rt, sl ^ HALF, k);
       }
-    if (i == i0) {
-      const __amdgpu_buffer_rsrc_t r = rsrc_of(i0);
-      load_k(r);
-      load_v(r);
     }
+  };
+  if (!SEQ || i0 < iend) {
+    issue_q(b, s);
+    const __amdgpu_buffer_rsrc_t r = rsrc_of(i0);
+    load_k(r);
+    load_v(r);
+  }
+  while (!SEQ || i0 < iend) {
+    float mxr[NRT], mxw = 0.0f;
+    // (of the largest |q| the bits: both halves of each word at once)
+    auto largest = [&](const uint4 &v, ushort2_t m) -> ushort2_t {
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(ushort2_t, word_of(v, w) & 0x7fff7fffu));
+      return m;
+    };
     if (own) prepare_new(b, s);
 #pragma unroll
     for (int rt = 0; rt < NRT; ++rt) {
-      float mx = 0.0f;
+      ushort2_t m2 = ushort2_t{0, 0};
 #pragma unroll
-      for (int k = 0; k < 2 * G; ++k) mx = largest(raw[rt][k], mx);
+      for (int k = 0; k < 2 * G; ++k) m2 = largest(raw[rt][k], m2);
+#pragma unroll
       for (int o = 1; o < DS; ++o)
 #pragma unroll
-        for (int k = 0; k < 2 * G; ++k) mx = largest(q_piece(rt, (sl + o) % DS, k), mx);
-      mx = fmaxf(mx, shfl_xor(mx, 16));
-      mx = fmaxf(mx, shfl_xor(mx, 32));
-      mxr[rt] = rvalid[rt] ? mx : 0.0f;
+        for (int k = 0; k < 2 * G; ++k) m2 = largest(q_piece(rt, (sl + o) % DS, k), m2);
+      int mb = max((int)m2[0], (int)m2[1]);
+      mb = max(mb, __shfl_xor(mb, 16, 64));
+      mb = max(mb, __shfl_xor(mb, 32, 64));
+      const float mx = a.q_dtype == DT_BF16 ? bf16_bits_to_f32((uint16_t)mb) : f16_bits_to_f32((uint16_t)mb);
+      mxr[rt] = rvalid[rt] && mx < INFINITY ? mx : 0.0f;
       mxw = fmaxf(mxw, mxr[rt]);
       if (a.rope_cs) {
         // dims d and d + D/2 turn together: in another slice's piece, this lane's
         // operand (head_dim 128) or lane ^ 32's (64)
-        const int j = (rvalid[rt] ? rbase + 16 * rt + n : 0) / a.R;
         const int len = WIN ? len_of(a, b) : seq_len(b);  // absolute positions
-        const float *crow = rope_row(a, len - a.Lq + j, D);
+        const float *crow = rope_row(a, len - a.Lq + rj[rt], D);
         uint4 old[2 * G];
 #pragma unroll
         for (int k = 0; k < 2 * G; ++k) old[k] = raw[rt][k];
@@ -465,30 +489,38 @@ __global__ __launch_bounds__(64 * (SEQ ? kSeqWaves : q4_slices<D>()), 2) void k_
         differ = true;
       }
       float qsum[G];
+      // !LOW: the codes come as 1024 + c and 1024 + 16 c, so pairs 1 and 3 are held
+      // over 16, and what is too much is where the products start from
+      const float f0 = rvalid[rt] ? ldexpf(1.0f, er) : 0.0f, f1 = LOW ? f0 : f0 * 0.0625f;
+      auto convert = [&](auto dtype) {
+        constexpr int DT = decltype(dtype)::value;
+        const half2_t one2 = half2_t{(_Float16)1.0f, (_Float16)1.0f};
+        const half2_t sixteen2 = half2_t{(_Float16)16.0f, (_Float16)16.0f};
+        const half2_t off2 = half2_t{(_Float16)-1024.0f, (_Float16)-1024.0f};
 #pragma unroll
-      for (int k = 0; k < 2 * G; ++k) {
-        if ((k & 1) == 0) qsum[k >> 1] = 0.0f;
-        half8_t v;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float x0 = ldexpf(elem(word_of(raw[rt][k], w), 0), er);
-          const float x1 = ldexpf(elem(word_of(raw[rt][k], w), 1), er);
-          v[2 * w] = rvalid[rt] ? (_Float16)x0 : (_Float16)0.0f;
-          v[2 * w + 1] = rvalid[rt] ? (_Float16)x1 : (_Float16)0.0f;
-          const float sum = (float)v[2 * w] + (float)v[2 * w + 1];
-          qsum[k >> 1] += sum;
-          if constexpr (!LOW) {
-            // (the codes come as 1024 + c and 1024 + 16 c: what is too much is
-            // where the products start from)
-            if (w & 1) {
-              v[2 * w] *= (_Float16)0.0625f;
-              v[2 * w + 1] *= (_Float16)0.0625f;
-            }
-            qoff[rt][k >> 1] = __builtin_fmaf((w & 1) ? -64.0f : -1024.0f, sum, k % 2 == 0 && w == 0 ? 0.0f : qoff[rt][k >> 1]);
+        for (int k = 0; k < 2 * G; ++k) {
+          if ((k & 1) == 0) {
+            qsum[k >> 1] = 0.0f;
+            if constexpr (!LOW) qoff[rt][k >> 1] = 0.0f;
           }
+          uint32_t h4[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t u = word_of(raw[rt][k], w);
+            const float f = (w & 1) ? f1 : f0;
+            const half2_t h = half2_t{(_Float16)(elem_to_f32<DT>((uint16_t)(u & 0xffffu)) * f),
+                                      (_Float16)(elem_to_f32<DT>((uint16_t)(u >> 16)) * f)};
+            qsum[k >> 1] = dot2(h, !LOW && (w & 1) ? sixteen2 : one2, qsum[k >> 1]);
+            if constexpr (!LOW) qoff[rt][k >> 1] = dot2(h, off2, qoff[rt][k >> 1]);
+            h4[w] = h2_as_u32(h);
+          }
+          qB[rt][k] = __builtin_bit_cast(half8_t, uint4{h4[0], h4[1], h4[2], h4[3]});
         }
-        qB[rt][k] = v;
-      }
+      };
+      if (a.q_dtype == DT_BF16)
+        convert(std::integral_constant<int, DT_BF16>{});
+      else
+        convert(std::integral_constant<int, DT_F16>{});
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         qsum[g] += shfl_xor(qsum[g], 16);
@@ -510,17 +542,15 @@ __global__ __launch_bounds__(64 * (SEQ ? kSeqWaves : q4_slices<D>()), 2) void k_
     int lim[NRT], lo[NRT], wst = 0, lo_hi = 0;
 #pragma unroll
     for (int rt = 0; rt < NRT; ++rt) {
-      const int r = rbase + 16 * rt + n;
-      lim[rt] = rvalid[rt] ? key_limit(a, len, r / a.R) : 0;
+      lim[rt] = rvalid[rt] ? key_limit(a, len, rj[rt]) : 0;
       lo[rt] = 0;
     }
-    const int lim_lo = key_limit(a, len, rbase / a.R);  // keys seen by the wave's first row
+    const int lim_lo = key_limit(a, len, j_first);  // keys seen by the wave's first row
     if constexpr (WIN) {
       wst = win_view_start(a, b);
 #pragma unroll
-      for (int rt = 0; rt < NRT; ++rt) lo[rt] = max(wst, len - a.Lq + (rbase + 16 * rt + n) / a.R - a.window + 1);
-      const int rlast = min(a.NR, rbase + RR) - 1;
-      lo_hi = max(wst, len - a.Lq + rlast / a.R - a.window + 1);
+      for (int rt = 0; rt < NRT; ++rt) lo[rt] = max(wst, len - a.Lq + rj[rt] - a.window + 1);
+      lo_hi = max(wst, len - a.Lq + j_last - a.window + 1);
     }
     float m_run[NRT], nm[NRT], l_part[NRT], c_part[NRT][G];
     float4_t o[NRT][NDT];
@@ -733,6 +763,15 @@ __global__ __launch_bounds__(64 * (SEQ ? kSeqWaves : q4_slices<D>()), 2) void k_
       wave_sync();  // (the metadata is read before the next block's is written)
     }
 
+    // the next sequence with blocks (the merge clears the others' rows)
+    int bn = b + 1;
+    bool more = false;
+    if (!SEQ && i < iend) {
+      while (bn < a.B && seq_blocks_rg(a, seq_len(bn), rg) == 0) ++bn;
+      more = bn < a.B;
+    }
+    if (more) issue_q(bn, e);
+
     // ---- the segment's end: lane holds O^T[16 dt + 4 q4 + x][row n]; output or a
     // partial in slot (hk row_groups + rg) (waves + B) + range + b
     const bool whole = !a.partial_only && s >= i0 && e <= iend;
@@ -772,7 +811,7 @@ __global__ __launch_bounds__(64 * (SEQ ? kSeqWaves : q4_slices<D>()), 2) void k_
       if (!rvalid[rt]) continue;
       const float mul = !whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
       const int64_t pi = slot * RR + 16 * rt + n;
-      const int64_t ob = (whole ? out_row_base(a, b, hk, rbase + 16 * rt + n, D) : pi * D) + sl * DW + 4 * q4;
+      const int64_t ob = (whole ? (((int64_t)b * a.Hq + hk * a.R + rh[rt]) * a.Lq + rj[rt]) * D : pi * D) + sl * DW + 4 * q4;
       auto put = [&](void *out, auto dtype) {
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
@@ -794,12 +833,9 @@ __global__ __launch_bounds__(64 * (SEQ ? kSeqWaves : q4_slices<D>()), 2) void k_
       if (!whole && sl == 0 && q4 == 0) reinterpret_cast<float2 *>(a.ws_ml)[pi] = float2{m_run[rt], l};
     }
     if (rg == 0 && new_phys >= 0) store_new(new_phys);
-    if (i >= iend) break;
-    // the next sequence with blocks (the merge clears the others' rows)
-    ++b;
+    if (!more) break;
+    b = bn;
     s = e;
-    while (b < a.B && seq_blocks_rg(a, seq_len(b), rg) == 0) ++b;
-    if (b >= a.B) break;
   }
 
   if constexpr (SEQ) {
