@@ -83,8 +83,6 @@ __device__ __forceinline__ uint32_t rest2(float w0, float w1, uint32_t h, float 
 // lanes' writes before other lanes' reads.
 __device__ __forceinline__ void wave_sync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
-
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
 __device__ __forceinline__ void set_word(uint4 &v, int w, uint32_t x) {
   (w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w) = x;

@@ -82,6 +82,91 @@ __device__ __forceinline__ uint32_t q4_code(float w, float s, float b, float r) 
   y = y < 15.0f ? y : 15.0f;
   return s > 0.0f ? (uint32_t)y : 0u;
 }
+// Eight elements (words of pairs of DT) of a group that eight lanes share (x, x ^ 1,
+// x ^ 2 and the half row's mirror): the group's metadata word and the codes, a byte
+// each.  Two forms of the same codes, the first for groups without infinities, NaN
+// and numbers past the fp16 range: rint(a / s) is taken from a r + 1.5 2^23, whose
+// low bits are the integer, and stands where what it leaves, a - n s, stays below
+// half a step by 2^-18 (the product with r is off by less than 2^-18 of a step);
+// ties, near ties and s = 0 take q4_code.
+__device__ __forceinline__ float q4_min3(float a, float b, float c) {
+  float r;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float q4_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float q4_max3_abs(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+template <int DT>
+__device__ __forceinline__ uint32_t q4_codes8(const uint32_t (&w4)[4], uint32_t &lo4, uint32_t &hi4) {
+  ushort2_t m2 = __builtin_bit_cast(ushort2_t, w4[0] & 0x7fff7fffu);
+#pragma unroll
+  for (int k = 1; k < 4; ++k) m2 = __builtin_elementwise_max(m2, __builtin_bit_cast(ushort2_t, w4[k] & 0x7fff7fffu));
+  const int top = max((int)m2[0], (int)m2[1]);
+  float w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = elem_to_f32<DT>((uint16_t)(w4[e >> 1] >> (16 * (e & 1))));
+  bool nan = false;
+  if (__any(top >= (DT == DT_BF16 ? 0x4780 : 0x7c00))) {  // 65536 in bf16, infinity in fp16
+    const int lane = threadIdx.x & 63;
+    nan = ((__ballot(top > (DT == DT_BF16 ? 0x7f80 : 0x7c00)) >> (lane & 56)) & 0xffull) != 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = w[e] != w[e] ? 0.0f : q4_limit<DT>(w[e]);  // (the group's codes do not matter then)
+  }
+  float lo = q4_min3(q4_min3(w[0], w[1], w[2]), w[3], w[4]), hi = q4_max3(q4_max3(w[0], w[1], w[2]), w[3], w[4]);
+  lo = q4_min3(q4_min3(lo, w[5], w[6]), w[7], dpp_f32<0xB1>(q4_min3(q4_min3(lo, w[5], w[6]), w[7], w[7])));
+  hi = q4_max3(q4_max3(hi, w[5], w[6]), w[7], dpp_f32<0xB1>(q4_max3(q4_max3(hi, w[5], w[6]), w[7], w[7])));
+  lo = fminf(lo, dpp_f32<0x4E>(lo));   // quad_perm [2,3,0,1]
+  hi = fmaxf(hi, dpp_f32<0x4E>(hi));
+  lo = fminf(lo, dpp_f32<0x141>(lo));  // row_half_mirror
+  hi = fmaxf(hi, dpp_f32<0x141>(hi));
+  float s, b;
+  const uint32_t meta = q4_params(lo, hi, nan, s, b);
+  const float r = __builtin_amdgcn_rcpf(s);
+  constexpr float M = 12582912.0f;
+  float t[8], off = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    float d[2];
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const float a = w[e + f] - b;
+      t[e + f] = __builtin_fmaf(a, r, M);
+      d[f] = __builtin_fmaf(M - t[e + f], s, a);
+    }
+    off = q4_max3_abs(off, d[0], d[1]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t[e] = __builtin_amdgcn_fmed3f(t[e], M, M + 15.0f);
+  // (a NaN among the t has one among the d, which v_max3 may pass over: s = 0 is
+  // asked for by itself)
+  if (__any(!(off < s * (0.5f - 0x1p-18f)) || !(s > 0.0f))) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = M + (float)q4_code(w[e], s, b, r);
+  }
+  uint32_t u[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) u[e] = __builtin_bit_cast(uint32_t, t[e]);
+  auto four = [&](int e) -> uint32_t {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[e + 3], u[e + 2], 0x0c0c0400u),
+                                 __builtin_amdgcn_perm(u[e + 1], u[e], 0x0c0c0400u), 0x05040100u);
+  };
+  lo4 = four(0);
+  hi4 = four(4);
+  return meta;
+}
+// the K word of eight codes
+__device__ __forceinline__ uint32_t q4_k_pack(uint32_t lo4, uint32_t hi4) {
+  return __builtin_amdgcn_perm(hi4, lo4, 0x05010400u) | (__builtin_amdgcn_perm(hi4, lo4, 0x07030602u) << 4);
+}
 // The value a code stands for, as the caches are read back: fp16, within its
 // range.
 __device__ __forceinline__ uint32_t q4_value_bits(uint32_t c, float s, float b) {

@@ -114,7 +114,6 @@ __global__ __launch_bounds__(256) void k_q4_append(LayerView lv, const uint16_t 
     im.slot[lane] = s;
     find_block<D>(im, s, lane);
   }
-  __syncthreads();
 
   const int x = lane % LPR;  // dims 8 x .. 8 x + 7
   const int64_t base = (int64_t)b * sb + (int64_t)h * sh + 8 * x;
@@ -132,8 +131,9 @@ __global__ __launch_bounds__(256) void k_q4_append(LayerView lv, const uint16_t 
     int row[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      // (rows without a slot are read too, so that no load waits for the slots)
       const int r = ((i0 + u) * 4 + wid) * RPW + lane / LPR;
-      row[u] = im.slot[r] >= 0 ? r : -1;
+      row[u] = r >= ra && r < rb ? r : -1;
       raw[u][0] = raw[u][1] = uint4{0u, 0u, 0u, 0u};
       if (row[u] >= 0) {
         const int64_t o = base + (int64_t)(l0 + r) * sl;
@@ -150,7 +150,8 @@ __global__ __launch_bounds__(256) void k_q4_append(LayerView lv, const uint16_t 
         if (ROPE && kv == 0) {
           // element i < D/2 pairs with i + D/2, LPR/2 lanes on; each product and
           // sum rounded once, then to the element type
-          const int p = r >= 0 ? rope.pos[(int64_t)b * L + l0 + r] : 0;
+          int p = r >= 0 ? rope.pos[(int64_t)b * L + l0 + r] : 0;
+          p = (unsigned)p < (unsigned)rope.max_pos ? p : 0;  // (outside: not written)
           const float *cs = rope.cs + (int64_t)p * D + 8 * (x % (LPR / 2));
           const bool hi = x >= LPR / 2;
 #pragma unroll
@@ -168,52 +169,19 @@ __global__ __launch_bounds__(256) void k_q4_append(LayerView lv, const uint16_t 
             w4[e] = res;
           }
         }
-        float w[8];
-        bool nan = false;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = elem_to_f32<DT>((uint16_t)(w4[e >> 1] >> (16 * (e & 1))));
-          nan |= y != y;
-          w[e] = q4_limit<DT>(y);
-        }
-        float lo = w[0], hi = w[0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) {
-          lo = fminf(lo, w[e]);
-          hi = fmaxf(hi, w[e]);
-        }
-        // over the group's eight lanes
-        lo = fminf(lo, dpp_f32<0xB1>(lo));   // quad_perm [1,0,3,2]
-        hi = fmaxf(hi, dpp_f32<0xB1>(hi));
-        lo = fminf(lo, dpp_f32<0x4E>(lo));   // quad_perm [2,3,0,1]
-        hi = fmaxf(hi, dpp_f32<0x4E>(hi));
-        lo = fminf(lo, dpp_f32<0x141>(lo));  // row_half_mirror
-        hi = fmaxf(hi, dpp_f32<0x141>(hi));
-        const bool any = ((__ballot(nan) >> (lane & 56)) & 0xffull) != 0;
-        float s, bias;
-        const uint32_t meta = q4_params(lo, hi, any, s, bias);
-        const float rs = __builtin_amdgcn_rcpf(s);
-        uint32_t code[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) code[e] = q4_code(w[e], s, bias, rs);
+        uint32_t lo4, hi4;
+        const uint32_t meta = q4_codes8<DT>(w4, lo4, hi4);
         if (kv == 0) {
-          uint32_t word = 0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) word |= code[e] << (4 * q4_nibble(e));
-          if (r >= 0) *reinterpret_cast<uint32_t *>(im.bytes + q4_k_word(D, r, x)) = word;
+          if (r >= 0) *reinterpret_cast<uint32_t *>(im.bytes + q4_k_word(D, r, x)) = q4_k_pack(lo4, hi4);
         } else {
           // bytes of dims (d, d + 16): the lane's and those of lane x ^ 2, four each
-          uint32_t a = 0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) a |= code[e] << (4 * e);
-          const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x4E, 0xf, 0xf, false);
           const bool up = (x & 2) != 0;
-          const uint32_t dl = (up ? o : a) >> (up ? 16 : 0), dh = (up ? a : o) >> (up ? 16 : 0);
+          const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(up ? lo4 : hi4), 0x4E, 0xf, 0xf, false);
+          const uint32_t v4 = up ? o | (hi4 << 4) : lo4 | (o << 4);
           const int m = 16 * (x >> 2) + 8 * (x & 1) + (up ? 4 : 0);
           if (r >= 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              im.bytes[q4_v_byte(D, r, m + e)] = (uint8_t)(((dl >> (4 * e)) & 15u) | (((dh >> (4 * e)) & 15u) << 4));
+            for (int e = 0; e < 4; ++e) im.bytes[q4_v_byte(D, r, m + e)] = (uint8_t)(v4 >> (8 * e));
           }
         }
         if (r >= 0 && (x & 7) == 0)
@@ -224,13 +192,31 @@ __global__ __launch_bounds__(256) void k_q4_append(LayerView lv, const uint16_t 
   __syncthreads();
 
   const int blk = im.block;
-  if (blk >= 0 && ra == 0 && rb == 64) {
-    if (__all(im.slot[lane] >= 0)) {
-      uint8_t *reg = head_region(lv, blk, h);
+  if (blk >= 0 && __all(lane < ra || lane >= rb || im.slot[lane] >= 0)) {
+    // a run of one block's tokens
+    uint8_t *reg = head_region(lv, blk, h);
+    if (ra == 0 && rb == 64) {
       for (int i = tid; i < q4_region_bytes(D) / 16; i += 256)
         reinterpret_cast<uint4 *>(reg)[i] = reinterpret_cast<const uint4 *>(im.bytes)[i];
       return;
     }
+    const int rows = rb - ra;
+    for (int i = tid; i < rows * (D / 16); i += 256)
+      move_row_item<D, true>(im.bytes, ra + i / (D / 16), reg, ra + i / (D / 16), i % (D / 16));
+    for (int i = tid; i < rows * 2 * G; i += 256)
+      move_row_item<D, true>(im.bytes, ra + i / (2 * G), reg, ra + i / (2 * G), D / 16 + D / 2 + i % (2 * G));
+    // V words of four tokens
+    for (int i = tid; i < 8 * D; i += 256) {
+      const int w = i & 3, t0 = 32 * (w >> 1) + 16 * (w & 1) + 4 * ((i >> 6) & 3), at = q4_v_offset(D) + 4 * i;
+      if (t0 >= ra && t0 + 4 <= rb) {
+        *reinterpret_cast<uint32_t *>(reg + at) = *reinterpret_cast<const uint32_t *>(im.bytes + at);
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (t0 + x >= ra && t0 + x < rb) reg[at + (q4_v_slot(x) & 3)] = im.bytes[at + (q4_v_slot(x) & 3)];
+      }
+    }
+    return;
   }
   for (int i = tid; i < (rb - ra) * row_items<D>(); i += 256) {
     const int r = ra + i / row_items<D>();
