@@ -1351,6 +1351,7 @@ int32_t plan_attention(const PoolGeometry &g, int32_t B, int32_t Hq, int32_t Lq,
 hipError_t launch_attn_merge(const PoolGeometry &g, int32_t layer, const AttnLaunch &a, const AttnPlan &p,
                              hipStream_t st) {
   if (a.B == 0) return hipSuccess;
+  if (p.q4 && (int64_t)p.NR * g.Hkv * a.B <= 4 * (int64_t)g.num_cus) return launch_q4_merge(g, layer, a, p, st);
   const AttnArgs args = make_attn_args(g, layer, a, p);
   // (few rows: one wave each, side by side; from 8192 on their workgroups are
   // what costs.  Whole calls by row groups over by rows, 693 of them: at 4096

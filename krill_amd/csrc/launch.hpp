@@ -149,6 +149,8 @@ hipError_t launch_attn_prefill(const PoolGeometry &g, int32_t layer, const AttnL
                                hipStream_t st);
 hipError_t launch_attn_q4(const PoolGeometry &g, int32_t layer, const AttnLaunch &a, const AttnPlan &p,
                           hipStream_t st);
+hipError_t launch_q4_merge(const PoolGeometry &g, int32_t layer, const AttnLaunch &a, const AttnPlan &p,
+                           hipStream_t st);
 hipError_t launch_attn_merge(const PoolGeometry &g, int32_t layer, const AttnLaunch &a, const AttnPlan &p,
                              hipStream_t st);
 
