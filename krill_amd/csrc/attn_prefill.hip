@@ -108,11 +108,19 @@ __device__ __forceinline__ void fence_lds() { __builtin_amdgcn_sched_barrier(0x4
 
 // Waves of a workgroup: one per (32-token group, 16-position half) of a V row.
 constexpr int kPrefillWaves = 4;
+// 4-bit pools at head_dim 128 and 256: twice as many waves share a converted
+// block, so each converts half as much (8 x 512 rows on 6000 tokens at head_dim
+// 128: 483 us against 498; 2 x 512 rows, window 1024, head_dim 256: 95 against
+// 110).  64 and 512 have no pieces or no LDS for it.
+template <int D, int MODE>
+constexpr int prefill_waves() {
+  return (MODE == MODE_AFFINE4 || MODE == MODE_DEQ4) && (D == 128 || D == 256) ? 8 : kPrefillWaves;
+}
 // Where in a head region the loads of a block lie: piece k of wave `wid` starts
 // at `piece` bytes (a scalar offset), each lane reads at its own offset from
 // there.  The range check of a buffer load does not cover the scalar offset, so
 // the sums must lie in the region by themselves.
-constexpr int prefill_k_piece(int wid, int k) { return (wid + kPrefillWaves * k) * 1024; }
+constexpr int prefill_k_piece(int wid, int k, int W = kPrefillWaves) { return (wid + W * k) * 1024; }
 template <int D>
 constexpr int prefill_v_piece(int wid, int k) {
   return v_offset(D) + ((wid >> 1) & 1) * 32 * D + (wid & 1) * 1024 + k * (64 / (D / 64) * 16);
@@ -123,9 +131,9 @@ constexpr int prefill_v_lane(int lane) { return 2 * (lane % (D / 64)) * 1024 + l
 // affine metadata, runs of 64 words: 128 G words, at G = 1 half of what the four
 // waves would load -- the other two read the same words again (unused)
 template <int D, int G>
-constexpr int prefill_meta_piece(int wid, int k) {
-  const int run = wid + kPrefillWaves * k;
-  return km_offset(D) + 256 * (2 * G < kPrefillWaves ? run % (2 * G) : run);
+constexpr int prefill_meta_piece(int wid, int k, int W = kPrefillWaves) {
+  const int run = wid + W * k;
+  return km_offset(D) + 256 * (2 * G < W ? run % (2 * G) : run);
 }
 template <int D, int G>
 constexpr bool prefill_loads_inside(int k_pieces, int v_pieces, int meta_pieces) {
@@ -147,24 +155,24 @@ constexpr int prefill_min_waves() { return NRT * D >= 512 ? 1 : 2; }
 
 // VAR: 0 plain; 1 RoPE of the queries; 2 sliding window.
 template <int D, int MODE, int NRT, int VAR>
-__global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_prefill(AttnArgs a) {
+__global__ __launch_bounds__((64 * prefill_waves<D, MODE>()), (prefill_min_waves<D, NRT>())) void k_attn_prefill(AttnArgs a) {
   constexpr bool ROPE = VAR == 1, WIN = VAR == 2, DEQ = MODE == MODE_DEQ4, AFF = MODE != MODE_REF && !DEQ,
                  Q4 = MODE == MODE_AFFINE4 || DEQ;
   constexpr int G = AFF ? D / 64 : 1;
   constexpr int GZ4 = (G + 3) / 4;
   constexpr int KS = D / 32;      // 32-d steps of Q.K^T
   constexpr int NDT = D / 16;     // 16-d tiles of P.V
-  constexpr int W = kPrefillWaves;
+  constexpr int W = prefill_waves<D, MODE>();
   constexpr int RR = 16 * NRT;    // query rows per wave
   // 16-byte pieces per thread of K and of V (4 bits: of both, wave wid the pieces
   // wid + W k of the region's D / 16, K's before V's)
   constexpr int KP = D / 16 / W;
   constexpr int VP = Q4 ? 0 : D / 16 / W;
   constexpr int GD = D / 64;      // scale groups of the pool's layout (4 bits)
-  constexpr int KQ = D / 64 >= 2 ? KP / 2 : KP;  // 4 bits: a thread's pieces that can be K's
-  constexpr int VM = (GD + 3) / 4;               // DEQ: words of V's metadata per thread
+  constexpr int KQ = KP >= 2 ? KP / 2 : KP;  // 4 bits: a thread's pieces that can be K's
+  constexpr int VM = (GD + W - 1) / W;       // DEQ: words of V's metadata per thread
   constexpr int MW = AFF ? (128 * G + 64 * W - 1) / (64 * W) : 0;  // metadata words per thread
-  static_assert(W == 4 && D % 64 == 0, "a wave per (token group, half) of V");
+  static_assert((Q4 || W == 4) && D % 64 == 0 && KP >= 1, "a wave per (token group, half) of V");
   static_assert(Q4 || prefill_loads_inside<D, G>(KP, VP, MW), "a block's loads stay in its head region");
   using Lds = PrefillLds<D, MODE>;
   constexpr int KTS = Lds::KTS, VTS = Lds::VTS;
@@ -246,7 +254,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
   uint4 kraw[KP], vraw[VP > 0 ? VP : 1];
   uint32_t mraw[AFF ? MW : 1];  // affine: words tid + 64 W k of the block's metadata; row mode: K word of token `lane`
   uint32_t vmeta = 0u;          // row mode: V word of token `lane`
-  uint32_t kword[DEQ ? KQ : 1][2], vword[DEQ ? VM : 1];  // DEQ: K's words of a piece's halves, V's words tid + 256 k
+  uint32_t kword[DEQ ? KQ : 1][2], vword[DEQ ? VM : 1];  // DEQ: K's words of a piece's halves, V's words tid + 64 W k
   const int vlane = prefill_v_lane<D>(lane);
   auto issue = [&](int i) {
     // after the last block: an empty resource (the offsets in scalars may escape
@@ -260,18 +268,18 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
       return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, soff, 0));
     };
 #pragma unroll
-    for (int k = 0; k < KP; ++k) kraw[k] = ld16(lane * 16, prefill_k_piece(wid, k));  // (4 bits: K's and V's)
+    for (int k = 0; k < KP; ++k) kraw[k] = ld16(lane * 16, prefill_k_piece(wid, k, W));  // (4 bits: K's and V's)
 #pragma unroll
     for (int k = 0; k < VP; ++k) vraw[k] = ld16(vlane, prefill_v_piece<D>(wid, k));
     if constexpr (AFF) {
 #pragma unroll
       for (int k = 0; k < MW; ++k)
         mraw[k] = __builtin_amdgcn_raw_buffer_load_b32(
-            r, lane * 4, prefill_meta_piece<D, G>(wid, k) - (Q4 ? km_offset(D) - q4_km_offset(D) : 0), 0);
+            r, lane * 4, prefill_meta_piece<D, G>(wid, k, W) - (Q4 ? km_offset(D) - q4_km_offset(D) : 0), 0);
     } else if constexpr (DEQ) {
 #pragma unroll
       for (int k = 0; k < VM; ++k)
-        vword[k] = __builtin_amdgcn_raw_buffer_load_b32(r, q4_vm_offset(D) + 4 * ((tid + 256 * k) & (64 * GD - 1)), 0, 0);
+        vword[k] = __builtin_amdgcn_raw_buffer_load_b32(r, q4_vm_offset(D) + 4 * ((tid + 64 * W * k) & (64 * GD - 1)), 0, 0);
 #pragma unroll
       for (int k = 0; k < KQ; ++k) {
         const int piece = (wid + W * k) & (D / 32 - 1);
@@ -292,7 +300,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
   auto stage_v = [&](int i) {
 #pragma unroll
     for (int k = 0; k < (DEQ ? VM : 0); ++k) {
-      const int m = tid + 256 * k, t = m / GD, g = m % GD, p = (t & 32) + vpos(t & 31);
+      const int m = tid + 64 * W * k, t = m / GD, g = m % GD, p = (t & 32) + vpos(t & 31);
       const float s = f16_bits_to_f32((uint16_t)(vword[k] & 0xffffu)), z = f16_bits_to_f32((uint16_t)(vword[k] >> 16));
       if (m < 64 * GD) {
         lds.ds[i & 1][64 * g + p] = (_Float16)(0.5f * s);
@@ -366,7 +374,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
         mx = fmaxf(mx, shfl_xor(mx, 32));
         down = q_range_scale(mx, up);
       }
-      if constexpr (!AFF) q_up[rt] = qscale * (DEQ ? fminf(up, 0x1p80f) : up);  // (DEQ: see below)
+      if constexpr (!AFF) q_up[rt] = qscale * (DEQ ? fminf(up, 0x1p80f) : up);
       // (4 bits: rows past about 2^95 take their scores some powers of two too small,
       // so that nothing overflows; scores that differ do so by far more than the
       // softmax resolves either way)
@@ -936,7 +944,7 @@ __global__ __launch_bounds__(256, (prefill_min_waves<D, NRT>())) void k_attn_pre
 
 template <int D, int MODE, int NRT>
 static hipError_t launch_prefill(const AttnArgs &args, unsigned groups, hipStream_t st) {
-  const dim3 grid((unsigned)args.waves * (unsigned)args.Hkv * groups), block(64 * kPrefillWaves);
+  const dim3 grid((unsigned)args.waves * (unsigned)args.Hkv * groups), block(64 * prefill_waves<D, MODE>());
   if (args.rope_cs) {  // (head_dim 512 comes here with several new rows only, RoPE with one)
     if constexpr (D <= 256)
       k_attn_prefill<D, MODE, NRT, 1><<<grid, block, 0, st>>>(args);
@@ -953,7 +961,7 @@ static hipError_t launch_prefill(const AttnArgs &args, unsigned groups, hipStrea
 template <int D, int MODE>
 static hipError_t launch_prefill_dm(const AttnArgs &args, const AttnPlan &p, hipStream_t st) {
   const unsigned groups = (unsigned)((p.row_groups + p.group_waves - 1) / p.group_waves);
-  if (p.group_waves != kPrefillWaves) return hipErrorInvalidValue;
+  if (p.group_waves != prefill_waves<D, MODE>()) return hipErrorInvalidValue;
   if (p.nrt == 1) return launch_prefill<D, MODE, 1>(args, groups, st);
   if constexpr (D <= 128) {
     if (p.nrt == 2) return launch_prefill<D, MODE, 2>(args, groups, st);
@@ -963,7 +971,10 @@ static hipError_t launch_prefill_dm(const AttnArgs &args, const AttnPlan &p, hip
 
 // Two waves per SIMD up to head_dim 256 (the registers), one at 512 (the
 // registers and 147 KB of LDS).
-int32_t prefill_groups_per_cu(const PoolGeometry &g) { return g.D >= 512 ? 1 : 2; }
+int32_t prefill_group_waves(const PoolGeometry &g) {
+  return g.mode == MODE_AFFINE4 && (g.D == 128 || g.D == 256) ? 8 : kPrefillWaves;
+}
+int32_t prefill_groups_per_cu(const PoolGeometry &g) { return g.D >= 512 ? 1 : 8 / prefill_group_waves(g); }
 
 hipError_t launch_attn_prefill(const PoolGeometry &g, int32_t layer, const AttnLaunch &a, const AttnPlan &p,
                                hipStream_t st) {

@@ -1214,7 +1214,7 @@ static int64_t prefill_ranges(int64_t cap, int64_t hg, int64_t tmax) {
 //                 4 x 100 on 100 37.1 / 31.1 (Hq 40)
 //   128, row      1 x 17 on 100 13.3 / 13.7; 1 x 48 on 1000 25.8 / 23.7
 static bool long_window_faster(const PoolGeometry &g, int64_t B, int64_t nb, int64_t NR, int64_t cus) {
-  const int64_t groups = ((NR + 15) / 16 + 3) / 4, tmax = B * nb;
+  const int64_t gw = prefill_group_waves(g), groups = ((NR + 15) / 16 + gw - 1) / gw, tmax = B * nb;
   const int64_t ranges = std::max<int64_t>(1, cus * prefill_groups_per_cu(g) / (g.Hkv * groups));
   const bool many = NR * g.Hkv * B > 4096;
   if (g.D > 256) return tmax > ranges || (many && 4 * tmax > ranges);
@@ -1276,12 +1276,12 @@ int32_t plan_attention(const PoolGeometry &g, int32_t B, int32_t Hq, int32_t Lq,
     // window 1024) and is not built.
     p.token_split = 1;
     if (p.prefill) {
-      const int64_t grp32 = ((p.NR + 31) / 32 + 3) / 4;
+      const int64_t gw = prefill_group_waves(g), grp32 = ((p.NR + 31) / 32 + gw - 1) / gw;
       const bool rows32 = g.D <= 128 && tmax >= 16 * (cus * prefill_groups_per_cu(g) / ((int64_t)g.Hkv * grp32));
       p.nrt = rows32 ? 2 : 1;
       p.rows_per_group = 16 * p.nrt;
       p.row_groups = (p.NR + p.rows_per_group - 1) / p.rows_per_group;
-      p.group_waves = 4;
+      p.group_waves = (int32_t)gw;
     } else if (p.NR > 16 && p.NR <= 32 && g.D <= 128) {
       p.nrt = 2;
       p.rows_per_group = 32;

@@ -128,7 +128,8 @@ int32_t valu_window_limit(const PoolGeometry &g, int32_t NR, bool rope);
 // occupancy query on a device pool.
 int32_t mfma_groups_per_cu(const PoolGeometry &g, int32_t group_waves, int32_t token_split);
 
-// Resident workgroups (four waves) per compute unit of the long-window kernel.
+// Waves of a workgroup of the long-window kernel, its resident workgroups per compute unit.
+int32_t prefill_group_waves(const PoolGeometry &g);
 int32_t prefill_groups_per_cu(const PoolGeometry &g);
 
 // 16-row tiles per wave and resident workgroups per compute unit of the 4-bit pools' kernel.
