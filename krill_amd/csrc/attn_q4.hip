@@ -30,6 +30,21 @@
 // Work split: the flat order of the int8 kernels -- per (KV head, row group) the
 // blocks of all sequences end to end, the same number to every wave -- and their
 // merge of partial results.
+//
+// Bound, measured with the step's append, RoPE and merge (head_dim, Hq / Hkv):
+//   few long contexts, 8 x 98304-131072 tokens (128, 32 / 4): the cache's reads,
+//     528 MB in 101 us, 5.2 TB/s (a large copy moves 4.8);
+//   32 x 512-8192 tokens (128, 40 / 8): 45.9 us for 157 MB; 39 us are this kernel,
+//     of them 5 before the first block is in and 10 while the last waves end;
+//   16 x 8 new rows on 1024-8192 tokens (128, 32 / 8): 41 us; conversion and
+//     softmax on the VALU, each unpacked operand feeds only two products;
+//   32 x 512-4096 tokens (512, 16 / 2): 45.8 us for 73 MB; the exchange of the
+//     scores' parts, a barrier a block, with one wave a SIMD;
+//   one sequence of 512 tokens (64, 32 / 8): 16 us, launches and the host.
+// Code runs once per call over tens of blocks, and an instruction costs about
+// 5.5 ns the first time it is fetched against 2 later: loops stay rolled where
+// they could be unrolled.  Three waves a SIMD spill: 61 us against 46 (the second
+// line above).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -98,7 +113,9 @@ constexpr float kGap = 5.0f, kOver = 8.0f, kBig = 255.0f;
 
 constexpr int kSeqWaves = 8, kSeqRows = 8;
 
-// Waves per SIMD the registers are budgeted for.
+// Waves per SIMD the registers are budgeted for.  Two row tiles at two waves spill
+// (16 x 8 new rows: 46.6 us as two row groups of one tile at two waves a SIMD, 40.8
+// as two tiles at one).
 template <int D, int NRT, bool SEQ>
 constexpr int q4_waves() { return NRT == 1 ? 2 : 1; }
 
@@ -968,7 +985,8 @@ int32_t q4_occupancy() {
 }  // namespace
 
 // Row tiles per wave: two from 17 rows on (each unpacked operand feeds two
-// products).
+// products): 32 rows take 40.8 us so, 46.6 as two groups of 16 that each read the
+// cache.  Up to 16 rows the second tile would be empty.
 int32_t q4_row_tiles(int32_t NR) { return NR > 16 ? 2 : 1; }
 
 int32_t q4_groups_per_cu(const PoolGeometry &g, int32_t nrt) {
@@ -981,6 +999,12 @@ int32_t q4_groups_per_cu(const PoolGeometry &g, int32_t nrt) {
   }
 }
 
+// A workgroup per (sequence, KV head), without a merge launch, while that many
+// workgroups find a CU each and a wave's share is at most three blocks: one
+// sequence of 512 tokens takes 16.6 us against 27.6 in the flat split (with less
+// time on the host, the same for both).  Longer contexts fill the card only when
+// they are split over it; a chosen split and the partials of a shared prefix need
+// the flat order.
 bool q4_per_sequence(const PoolGeometry &g, const AttnLaunch &a, const AttnPlan &p) {
   if (!p.q4 || g.D > 128 || p.NR > kSeqRows || p.split_blocks > 0 || a.partial_only || a.len_const >= 0 || !a.causal)
     return false;

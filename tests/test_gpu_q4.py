@@ -731,3 +731,88 @@ def test_long_windows_with_bf16_outputs(D, Lq, R, window):
     got[1, 0, Lq // 2] = clean[1, 0, Lq // 2]
     same(got.float().cpu().numpy(), clean.float().cpu().numpy())
     pool.close()
+
+
+@pytest.mark.parametrize("L", [1, 17])
+def test_append_of_more_sequences_than_a_grid_dimension(L):
+    """A batch past 65535 rows of slots, nearly all of them skipped."""
+    rng = np.random.default_rng(L)
+    B, H, D, blocks = 65536 + 5, 1, 64, 4
+    pool = make_pool(H, D, blocks)
+    kb = np.zeros((B, H, L, D), np.uint16)
+    vb = np.zeros_like(kb)
+    slots = np.full((B, L), -1, np.int32)
+    for i, b in enumerate((0, 40000, 65535, 65536, B - 1)):
+        kb[b], vb[b] = rand_bits(rng, (H, L, D), "bf16"), rand_bits(rng, (H, L, D), "bf16")
+        slots[b] = 1 + 40 * i + np.arange(L)
+    pool.quantize_append(0, to_dev(kb, "bf16"), to_dev(vb, "bf16"), i32(slots))
+    want = np.zeros((2, H, blocks * 64, D), np.float16)
+    for b in np.flatnonzero(slots[:, 0] >= 0):
+        want[0][:, slots[b]] = Q.read_back(Q.stored(kb[b], "bf16"))
+        want[1][:, slots[b]] = Q.read_back(Q.stored(vb[b], "bf16"))
+    k, v = pool.read_slots(0, all_slots(pool))
+    same(k[0].cpu().numpy(), want[0])
+    same(v[0].cpu().numpy(), want[1])
+    pool.close()
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("D,R,chunk", [(64, 4, 96), (128, 5, 64), (256, 2, 33)])
+def test_batcher_over_a_4bit_pool(D, R, chunk, out):
+    """Requests that come and go: chunked prefill, batched decode steps, blocks given back and reused; every
+    output of every request and layer against 64 bits over that request's own tokens."""
+    from krill_amd.batcher import ContinuousBatcher, Request
+
+    H, layers, dt = 2, 2, "bf16"
+    reqs = [Request(rid, T, g) for rid, T, g in [(0, 70, 5), (1, 5, 9), (2, 130, 3), (3, 64, 6), (4, 1, 4), (5, 200, 2)]]
+    arrivals = {0: reqs[:2], 1: reqs[2:3], 4: reqs[3:5], 6: reqs[5:]}
+
+    class Model:
+        def __init__(self):
+            self.x, self.out = {}, {}
+            for r in reqs:
+                rng, T = np.random.default_rng(r.rid + D), r.prompt_len + r.max_new_tokens
+                for l in range(layers):
+                    self.x[r.rid, l] = [rand_bits(rng, (n, T, D), dt) for n in (H * R, H, H)]
+                    self.out[r.rid, l] = np.full((H * R, T, D), np.nan)
+
+        def prefill(self, req, start, n, layer):
+            return tuple(to_dev(a[None, :, start:start + n], dt) for a in self.x[req.rid, layer])
+
+        def decode(self, rs, positions, layer):
+            return tuple(to_dev(np.stack([self.x[r.rid, layer][i][:, p:p + 1] for r, p in zip(rs, positions)]), dt)
+                         for i in range(3))
+
+        def consume(self, rs, layer, positions, o):
+            o = o.float().cpu().numpy()
+            if len(rs) == 1:
+                self.out[rs[0].rid, layer][:, positions] = o[0]
+            else:
+                for b, (r, p) in enumerate(zip(rs, positions)):
+                    self.out[r.rid, layer][:, p] = o[b, :, 0]
+
+    pool = make_pool(H, D, 16, dt, layers)
+    model, scale = Model(), D ** -0.5
+    cb = ContinuousBatcher(pool, model, 3, H * R, scale, prefill_chunk=chunk,
+                           out_dtype=torch.float32 if out == "f32" else torch.bfloat16)
+    for step in range(100):
+        for r in arrivals.get(step, []):
+            cb.submit(r)
+        if cb.idle and step > max(arrivals):
+            break
+        cb.step()
+    torch.cuda.synchronize()
+    assert cb.idle
+    for r in reqs:
+        T = r.prompt_len + r.max_new_tokens
+        for l in range(layers):
+            qb, kb, vb = model.x[r.rid, l]
+            qf = O.bits_to_f32(qb, Q.DT[dt]).astype(np.float64)
+            for h in range(H):
+                kd, vd = Q.stored(kb[h], dt), Q.stored(vb[h], dt)
+                rows, hi = qf[h * R:(h + 1) * R].reshape(R * T, D), np.tile(np.arange(1, T + 1), R)
+                want = Q.attention(rows, kd, vd, np.zeros_like(hi), hi, scale)
+                got = model.out[r.rid, l][h * R:(h + 1) * R].reshape(R * T, D)
+                lim = Q.bound(rows, kd, vd, scale, want, out, *(Q.quantize(x[h], dt)[1].max() for x in (kb, vb)), long=True)
+                assert np.all(np.abs(got - want) <= lim), f"request {r.rid} layer {l} head {h}"
+    pool.close()
