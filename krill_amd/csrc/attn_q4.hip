@@ -34,11 +34,11 @@
 // Bound, measured with the step's append, RoPE and merge (head_dim, Hq / Hkv):
 //   few long contexts, 8 x 98304-131072 tokens (128, 32 / 4): the cache's reads,
 //     528 MB in 101 us, 5.2 TB/s (a large copy moves 4.8);
-//   32 x 512-8192 tokens (128, 40 / 8): 45.9 us for 157 MB; 39 us are this kernel,
+//   32 x 512-8192 tokens (128, 40 / 8): 45.7 us for 161 MB; 38 us are this kernel,
 //     of them 5 before the first block is in and 10 while the last waves end;
 //   16 x 8 new rows on 1024-8192 tokens (128, 32 / 8): 41 us; conversion and
 //     softmax on the VALU, each unpacked operand feeds only two products;
-//   32 x 512-4096 tokens (512, 16 / 2): 45.8 us for 73 MB; the exchange of the
+//   32 x 512-4096 tokens (512, 16 / 2): 45.7 us for 87 MB; the exchange of the
 //     scores' parts, a barrier a block, with one wave a SIMD;
 //   one sequence of 512 tokens (64, 32 / 8): 16 us, launches and the host.
 // Code runs once per call over tens of blocks, and an instruction costs about
