@@ -111,7 +111,8 @@ constexpr int kPrefillWaves = 4;
 // 4-bit pools at head_dim 128 and 256: twice as many waves share a converted
 // block, so each converts half as much (8 x 512 rows on 6000 tokens at head_dim
 // 128: 483 us against 498; 2 x 512 rows, window 1024, head_dim 256: 95 against
-// 110).  64 and 512 have no pieces or no LDS for it.
+// 110; the exact form for fp16 outputs: 238 -> 235 at 256, 739 -> 747 at 128).  64
+// and 512 have no pieces or no LDS for it.
 template <int D, int MODE>
 constexpr int prefill_waves() {
   return (MODE == MODE_AFFINE4 || MODE == MODE_DEQ4) && (D == 128 || D == 256) ? 8 : kPrefillWaves;
@@ -945,8 +946,9 @@ __global__ __launch_bounds__((64 * prefill_waves<D, MODE>()), (prefill_min_waves
 template <int D, int MODE, int NRT>
 static hipError_t launch_prefill(const AttnArgs &args, unsigned groups, hipStream_t st) {
   const dim3 grid((unsigned)args.waves * (unsigned)args.Hkv * groups), block(64 * prefill_waves<D, MODE>());
-  if (args.rope_cs) {  // (head_dim 512 comes here with several new rows only, RoPE with one)
-    if constexpr (D <= 256)
+  // (head_dim 512 and 4-bit pools come here with several new rows only, RoPE with one)
+  if (args.rope_cs) {
+    if constexpr (D <= 256 && (MODE == MODE_REF || MODE == MODE_AFFINE))
       k_attn_prefill<D, MODE, NRT, 1><<<grid, block, 0, st>>>(args);
     else
       return hipErrorInvalidValue;

@@ -816,3 +816,36 @@ def test_batcher_over_a_4bit_pool(D, R, chunk, out):
                 lim = Q.bound(rows, kd, vd, scale, want, out, *(Q.quantize(x[h], dt)[1].max() for x in (kb, vb)), long=True)
                 assert np.all(np.abs(got - want) <= lim), f"request {r.rid} layer {l} head {h}"
     pool.close()
+
+
+@pytest.mark.parametrize("out", ["bf16", "f16"])
+@pytest.mark.parametrize("Lq,R,path,split", [(2, 1, 2, 0), (9, 5, 2, 0), (9, 5, 2, 1), (70, 2, 1, 0), (70, 2, 0, 1)])
+@pytest.mark.parametrize("window", [2, 100])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_windows_on_chosen_paths(D, window, Lq, R, path, split, out):
+    """Sliding windows on the kernel and the block ranges a caller asks for."""
+    from krill_amd import _lib as L
+
+    rng = np.random.default_rng(window * Lq + D)
+    H, dt, scale = 2, "bf16", 1 / np.sqrt(D)
+    lens = [Lq, 130 + Lq, 331]
+    pool = make_pool(H, D, 30, dt)
+    for o, x in ((L.OPT_WINDOW, window), (L.OPT_ATTN_PATH, path), (L.OPT_SPLIT_BLOCKS, split)):
+        pool.set_option(o, x)
+    kb = [rand_bits(rng, (H, T, D), dt) for T in lens]
+    vb = [rand_bits(rng, (H, T, D), dt) for T in lens]
+    seqs = [pool.seq_create() for _ in lens]
+    for b, T in enumerate(lens):
+        for t0, t1 in ((0, T - Lq), (T - Lq, T)):
+            if t1 > t0:
+                sl = pool.reserve_append(seqs[b], t1 - t0)
+                pool.quantize_append(0, to_dev(kb[b][None, :, t0:t1], dt), to_dev(vb[b][None, :, t0:t1], dt), i32(sl[None]))
+    tab, n = pool.batch_tables(seqs, 6)
+    starts = i32(pool.batch_starts(seqs))
+    qb = rand_bits(rng, (len(lens), H * R, Lq, D), dt)
+    c = Cache.__new__(Cache)
+    c.pool, c.lens, c.dt, c.k, c.v = pool, lens, dt, kb, vb
+    got = pool.attention_windowed(0, to_dev(qb, dt), i32(tab), i32(n), starts, window, max(lens), scale,
+                                  out_dtype={"bf16": torch.bfloat16, "f16": torch.float16}[out])
+    c.check(got, qb, scale, out, window, long=True)
+    pool.close()
